@@ -94,6 +94,19 @@ _SIGNATURES = {
     "gx_argmax_step": [_vp, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp],
     "gx_argmax_slots_step": [_vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp],
     "gx_argmax": [_vp, _vp, _c_int, _c_int, _c_int, _vp],
+    "gx_qwen_tree_plan": [_vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp,
+                          _vp],
+    "gx_qwen_attention_tree_workspace_bytes": [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                               ctypes.POINTER(_c_size)],
+    "gx_qwen_attention_tree": [_vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp,
+                               _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_size, _vp, _c_int],
+    "gx_tree_verify_workspace_bytes": [_c_int, _c_int, _c_int, ctypes.POINTER(_c_size)],
+    "gx_tree_verify": [_vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _c_int, ctypes.c_float,
+                       ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _c_size],
+    "gx_qwen_cache_commit": [_vp, _c_int, _pp, _pp, _pp, _pp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _c_int,
+                             _c_int, _c_int, _c_int, _vp, _c_int],
+    "gx_qwen_cache_fork": [_vp, _c_int, _pp, _pp, _c_int, _c_int, _c_int, _c_int, _c_int,
+                           ctypes.POINTER(ctypes.c_int32), _c_int, _c_int],
     "gx_geglu_quant": [_vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp],
     "gx_moe_join": [_vp, _vp, _c_int, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, ctypes.c_float, _vp,
                     _c_int],

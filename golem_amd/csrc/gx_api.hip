@@ -1083,6 +1083,193 @@ int gx_argmax_slots_step(gx_ctx *ctx, const float *x, int ldx, int M, int n, int
     return ok();
 }
 
+// ---- drafted trees ---------------------------------------------------------
+//
+// (the arguments are checked before the context, so that a misuse is named
+// without a GPU too)
+
+static int check_trees(int n, int M, int max_nodes) {
+    GX_CHECK(n >= 0 && n <= gx::kTrees, "gx: %d trees (at most %d)", n, gx::kTrees);
+    GX_CHECK(M >= 0 && M <= 65535, "gx: %d tokens (at most 65535)", M);
+    GX_CHECK(max_nodes > 0 && max_nodes <= gx::kTreeNodes, "gx: trees of %d nodes (1 to %d)", max_nodes,
+             gx::kTreeNodes);
+    return GX_OK;
+}
+
+int gx_qwen_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *first, const int32_t *parents,
+                      const int32_t *prefix, const float *rope_cos, const float *rope_sin, int half, int context,
+                      int32_t *rows, int32_t *positions, uint32_t *mask, float *cos, float *sin) {
+    if (int rc = check_trees(n, M, max_nodes))
+        return rc;
+    GX_CHECK(half > 0 && context > 0, "gx: rotation tables of %d rows of %d", context, half);
+    GX_CHECK(first && parents && prefix && rope_cos && rope_sin && rows && positions && mask && cos && sin,
+             "gx: missing argument");
+    if (int rc = use(ctx))
+        return rc;
+    if (M == 0)
+        return ok();
+    if (int rc = gx::launch_tree_plan(ctx, n, M, max_nodes, first, parents, prefix, rope_cos, rope_sin, half, context,
+                                      rows, positions, mask, cos, sin))
+        return rc;
+    return ok();
+}
+
+static int check_tree_heads(int heads, int kv_heads, int head_dim, int max_prefix) {
+    GX_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "gx: %d query heads over %d key-value heads", heads,
+             kv_heads);
+    GX_CHECK(heads <= 4096, "gx: %d query heads (at most 4096)", heads);
+    GX_CHECK(head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128,
+             "gx: attention supports head widths 32, 64, 96 and 128");
+    GX_CHECK(max_prefix >= 0, "gx: a prefix of %d", max_prefix);
+    return GX_OK;
+}
+
+int gx_qwen_attention_tree_workspace_bytes(int n, int M, int max_nodes, int heads, int kv_heads, int head_dim,
+                                           int max_prefix, size_t *bytes) {
+    GX_CHECK(bytes != nullptr, "gx: no place for the size");
+    if (int rc = check_trees(n, M, max_nodes))
+        return rc;
+    if (int rc = check_tree_heads(heads, kv_heads, head_dim, max_prefix))
+        return rc;
+    *bytes = gx::attn_tree_workspace(n, M, max_nodes, heads, kv_heads, head_dim, max_prefix);
+    return ok();
+}
+
+int gx_qwen_attention_tree(gx_ctx *ctx, const uint16_t *qh, int n, int M, int max_nodes, const int32_t *first,
+                           const uint32_t *mask, const int32_t *prefix, int max_prefix, int heads, int kv_heads,
+                           int head_dim, const uint16_t *kcache, const uint16_t *vcache, int context,
+                           const uint16_t *kdraft, const uint16_t *vdraft, int draft_context, float *out, int8_t *q,
+                           float *scales, int32_t *qsum, void *workspace, size_t workspace_bytes,
+                           const int32_t *slots, int nslots) {
+    if (int rc = check_trees(n, M, max_nodes))
+        return rc;
+    if (int rc = check_tree_heads(heads, kv_heads, head_dim, max_prefix))
+        return rc;
+    GX_CHECK(context > 0 && context % 8 == 0 && max_prefix <= context,
+             "gx: a cache of %d positions (a multiple of 8) cannot hold %d", context, max_prefix);
+    GX_CHECK(draft_context > 0 && draft_context % 8 == 0 && draft_context >= M,
+             "gx: draft buffers of %d rows (a multiple of 8) cannot hold %d", draft_context, M);
+    GX_CHECK((int64_t)context * head_dim <= INT32_MAX && (int64_t)draft_context * head_dim <= INT32_MAX,
+             "gx: a head of %d positions is too long", context > draft_context ? context : draft_context);
+    GX_CHECK(qh && first && mask && prefix && kcache && vcache && kdraft && vdraft && (out || q) &&
+                 (!q || (scales && qsum)) && workspace,
+             "gx: missing argument");
+    GX_CHECK((((uintptr_t)qh | (uintptr_t)kcache | (uintptr_t)vcache | (uintptr_t)kdraft | (uintptr_t)vdraft) & 15) == 0,
+             "gx: the queries, the caches and the draft buffers must be 16-byte aligned");
+    GX_CHECK(((uintptr_t)workspace & 255) == 0, "gx: the workspace must be 256-byte aligned");
+    GX_CHECK(!slots || nslots > 0, "gx: %d slots", nslots);
+    const size_t need = gx::attn_tree_workspace(n, M, max_nodes, heads, kv_heads, head_dim, max_prefix);
+    GX_CHECK(workspace_bytes >= need, "gx: the workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+    if (int rc = use(ctx))
+        return rc;
+    if (n == 0 || M == 0)
+        return ok();
+    const gx::TreeAttention y{qh,       n,        M,        max_nodes, first,  mask,    prefix, max_prefix,    heads,
+                              kv_heads, head_dim, kcache,   vcache,    context, kdraft, vdraft, draft_context, slots,
+                              nslots};
+    if (int rc = gx::launch_attn_tree(ctx, y, out, q, scales, qsum, (uint8_t *)workspace))
+        return rc;
+    return ok();
+}
+
+int gx_tree_verify_workspace_bytes(int n, int M, int vocab, size_t *bytes) {
+    GX_CHECK(bytes != nullptr, "gx: no place for the size");
+    if (int rc = check_trees(n, M, 1))
+        return rc;
+    GX_CHECK(vocab > 0 && vocab <= gx::kVocabMax, "gx: a vocabulary of %d (at most %d)", vocab, gx::kVocabMax);
+    *bytes = gx::tree_verify_workspace(n, M, vocab);
+    return ok();
+}
+
+int gx_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
+                   const int32_t *first, const int32_t *parents, const int32_t *tokens, const float *draft_logits,
+                   int ldd, float temperature, float draft_temperature, const float *uniforms, int32_t *path,
+                   int32_t *counts, int32_t *next, void *workspace, size_t workspace_bytes) {
+    if (int rc = check_trees(n, M, max_nodes))
+        return rc;
+    GX_CHECK(vocab > 0 && vocab <= gx::kVocabMax, "gx: a vocabulary of %d (at most %d)", vocab, gx::kVocabMax);
+    GX_CHECK(ldl >= vocab && (!draft_logits || ldd >= vocab), "gx: bad shape");
+    GX_CHECK(temperature >= 0.0f && temperature <= 3.0e38f, "gx: a temperature of %g", (double)temperature);
+    GX_CHECK(!draft_logits || temperature == 0.0f || (draft_temperature > 0.0f && draft_temperature <= 3.0e38f),
+             "gx: a draft temperature of %g", (double)draft_temperature);
+    GX_CHECK(logits && first && parents && tokens && path && counts && next && workspace &&
+                 (uniforms || temperature == 0.0f),
+             "gx: missing argument");
+    GX_CHECK(((uintptr_t)workspace & 255) == 0, "gx: the workspace must be 256-byte aligned");
+    const size_t need = gx::tree_verify_workspace(n, M, vocab);
+    GX_CHECK(workspace_bytes >= need, "gx: the workspace holds %zu bytes, %zu needed", workspace_bytes, need);
+    if (int rc = use(ctx))
+        return rc;
+    if (n == 0)
+        return ok();
+    if (int rc = gx::launch_tree_verify(ctx, logits, ldl, n, M, max_nodes, vocab, first, parents, tokens, draft_logits,
+                                        ldd, temperature, draft_temperature, uniforms, path, counts, next,
+                                        (uint8_t *)workspace))
+        return rc;
+    return ok();
+}
+
+static int check_layers(int layers, int kv_heads, int head_dim, int context, uint16_t *const *kcaches,
+                        uint16_t *const *vcaches) {
+    GX_CHECK(layers > 0 && kv_heads > 0 && kv_heads <= 65535 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= 1024,
+             "gx: caches of %d layers, %d key-value heads of %d", layers, kv_heads, head_dim);
+    GX_CHECK(context > 0 && context % 8 == 0, "gx: a cache of %d positions (a multiple of 8)", context);
+    GX_CHECK(kcaches && vcaches, "gx: missing argument");
+    for (int l = 0; l < layers; l++)
+        GX_CHECK(kcaches[l] && vcaches[l] && (((uintptr_t)kcaches[l] | (uintptr_t)vcaches[l]) & 15) == 0,
+                 "gx: the caches of layer %d must be 16-byte aligned device memory", l);
+    return GX_OK;
+}
+
+int gx_qwen_cache_commit(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches,
+                         const uint16_t *const *kdrafts, const uint16_t *const *vdrafts, int n, int M, int max_nodes,
+                         const int32_t *first, const int32_t *path, const int32_t *counts, const int32_t *prefix,
+                         int kv_heads, int head_dim, int context, int draft_context, const int32_t *slots,
+                         int nslots) {
+    if (int rc = check_trees(n, M, max_nodes))
+        return rc;
+    if (int rc = check_layers(layers, kv_heads, head_dim, context, kcaches, vcaches))
+        return rc;
+    GX_CHECK(draft_context > 0 && draft_context % 8 == 0 && draft_context >= M,
+             "gx: draft buffers of %d rows (a multiple of 8) cannot hold %d", draft_context, M);
+    GX_CHECK(kdrafts && vdrafts && first && path && counts && prefix, "gx: missing argument");
+    for (int l = 0; l < layers; l++)
+        GX_CHECK(kdrafts[l] && vdrafts[l] && (((uintptr_t)kdrafts[l] | (uintptr_t)vdrafts[l]) & 15) == 0,
+                 "gx: the draft buffers of layer %d must be 16-byte aligned device memory", l);
+    GX_CHECK(!slots || nslots > 0, "gx: %d slots", nslots);
+    if (int rc = use(ctx))
+        return rc;
+    if (n == 0 || M == 0)
+        return ok();
+    if (int rc = gx::launch_cache_commit(ctx, layers, kcaches, vcaches, kdrafts, vdrafts, n, M, max_nodes, first, path,
+                                         counts, prefix, kv_heads, head_dim, context, draft_context, slots,
+                                         slots ? nslots : 1))
+        return rc;
+    return ok();
+}
+
+int gx_qwen_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches, int nslots,
+                       int kv_heads, int head_dim, int context, int src, const int32_t *dsts, int n, int len) {
+    if (int rc = check_layers(layers, kv_heads, head_dim, context, kcaches, vcaches))
+        return rc;
+    GX_CHECK(nslots > 0 && src >= 0 && src < nslots, "gx: slot %d of %d", src, nslots);
+    GX_CHECK(n >= 0 && n < nslots && (n == 0 || dsts), "gx: %d forks among %d slots", n, nslots);
+    GX_CHECK(len >= 0 && len <= context, "gx: %d positions of a cache of %d", len, context);
+    for (int i = 0; i < n; i++) {
+        GX_CHECK(dsts[i] >= 0 && dsts[i] < nslots, "gx: slot %d of %d", dsts[i], nslots);
+        GX_CHECK(dsts[i] != src, "gx: slot %d forked into itself", src);
+        for (int j = 0; j < i; j++)
+            GX_CHECK(dsts[i] != dsts[j], "gx: slot %d named twice", dsts[i]);
+    }
+    if (int rc = use(ctx))
+        return rc;
+    if (n == 0 || len == 0)
+        return ok();
+    if (int rc = gx::launch_cache_fork(ctx, layers, kcaches, vcaches, kv_heads, head_dim, context, src, dsts, n, len))
+        return rc;
+    return ok();
+}
+
 static int moe_experts(gx_ctx *ctx, const gx_weight *gate_up, const gx_weight *down, const float *down_scale,
                        const float *x, int ldx, int M, int top_k, const int32_t *ids, const float *weights, float *out,
                        int ldo, void *workspace, size_t workspace_bytes, bool noalloc) {

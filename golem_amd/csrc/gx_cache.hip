@@ -1,0 +1,133 @@
+// gx_cache.hip - a conversation's cache entries moved as a whole: a kept path's
+// draft entries into the caches, and a conversation's first positions into
+// other slots.  Every layer in one launch: the layers' addresses are kernel
+// arguments.  Bytes alone, read once.
+#include "gx_device.hpp"
+#include "gx_internal.hpp"
+
+namespace gx {
+namespace {
+
+struct CommitLayers {
+    uint16_t *kc[kCacheLayers], *vc[kCacheLayers];
+    const uint16_t *kd[kCacheLayers], *vd[kCacheLayers];
+};
+
+// grid (kv_heads, trees, layers): node path[b][j] of tree b, draft row first[b]
+// + that, becomes position prefix[b] + j of its conversation.  A node or a
+// position out of range is left out.
+__global__ __launch_bounds__(256) void cache_commit_kernel(const CommitLayers at, int M, int max_nodes,
+                                                           const int32_t *__restrict__ first,
+                                                           const int32_t *__restrict__ path,
+                                                           const int32_t *__restrict__ counts,
+                                                           const int32_t *__restrict__ prefix, int hd, int context,
+                                                           int draft_context, const int32_t *__restrict__ slots,
+                                                           int nslots) {
+    __shared__ int from[kTreeNodes];
+    const int tid = threadIdx.x, kvh = blockIdx.x, kv_heads = gridDim.x, b = blockIdx.y, layer = blockIdx.z;
+    const int f0 = min(max(first[b], 0), M), T = min(min(max(first[b + 1], f0), M) - f0, max_nodes);
+    const int count = min(max(counts[b], 0), max_nodes), p0 = prefix[b], slot = slots ? slots[b] : 0;
+    if (slot < 0 || slot >= nslots || p0 < 0 || p0 >= context)
+        return;
+    for (int j = tid; j < count; j += 256) {
+        const int node = path[(size_t)b * max_nodes + j];
+        from[j] = node >= 0 && node < T && p0 < context - j ? f0 + node : -1;
+    }
+    __syncthreads();
+    const size_t to = ((size_t)slot * kv_heads + kvh) * hd * context, src = (size_t)kvh * hd * draft_context;
+    v4u_stream *kc = (v4u_stream *)(at.kc[layer] + to);
+    const v4u_stream *kd = (const v4u_stream *)(at.kd[layer] + src);
+    for (int i = tid; i < hd / 8 * count; i += 256) {
+        const int e = i / count, j = i - e * count;
+        if (from[j] >= 0)
+            kc[(size_t)e * context + p0 + j] = kd[(size_t)e * draft_context + from[j]];
+    }
+    uint16_t *vc = at.vc[layer] + to;
+    const uint16_t *vd = at.vd[layer] + src;
+    for (int i = tid; i < hd * count; i += 256) {
+        const int e = i / count, j = i - e * count;
+        if (from[j] >= 0)
+            vc[(size_t)e * context + p0 + j] = vd[(size_t)e * draft_context + from[j]];
+    }
+}
+
+struct ForkLayers {
+    uint16_t *kc[kCacheLayers], *vc[kCacheLayers];
+    int dsts[kForkSlots];
+};
+
+// grid (kv_heads * hd / 8, 2, layers): a piece row of the keys (y 0, 16 bytes a
+// position) or eight element rows of the values.
+__global__ __launch_bounds__(256) void cache_fork_kernel(const ForkLayers at, int kv_heads, int hd, int context,
+                                                         int src, int n, int len) {
+    const int tid = threadIdx.x, layer = blockIdx.z;
+    const size_t slot = (size_t)kv_heads * hd * context;
+    if (blockIdx.y == 0) {
+        v4u_stream *k = (v4u_stream *)(at.kc[layer] + (size_t)blockIdx.x * 8 * context);
+        for (int i = tid; i < len; i += 256) {
+            const v4u_stream v = k[src * (slot / 8) + i];
+            for (int d = 0; d < n; d++)
+                k[at.dsts[d] * (slot / 8) + i] = v;
+        }
+        return;
+    }
+    for (int r = 0; r < 8; r++) {
+        uint16_t *vr = at.vc[layer] + ((size_t)blockIdx.x * 8 + r) * context;
+        for (int i = tid; i < len / 8; i += 256) {
+            const v4u_stream v = ((const v4u_stream *)(vr + src * slot))[i];
+            for (int d = 0; d < n; d++)
+                ((v4u_stream *)(vr + at.dsts[d] * slot))[i] = v;
+        }
+        // positions from len on stay the slot's own
+        const int i = len / 8 * 8 + tid;
+        if (i < len)
+            for (int d = 0; d < n; d++)
+                vr[at.dsts[d] * slot + i] = vr[src * slot + i];
+    }
+}
+
+}  // namespace
+
+int launch_cache_commit(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches,
+                        const uint16_t *const *kdrafts, const uint16_t *const *vdrafts, int n, int M, int max_nodes,
+                        const int32_t *first, const int32_t *path, const int32_t *counts, const int32_t *prefix,
+                        int kv_heads, int hd, int context, int draft_context, const int32_t *slots, int nslots) {
+    for (int l0 = 0; l0 < layers; l0 += kCacheLayers) {
+        const int here = layers - l0 < kCacheLayers ? layers - l0 : kCacheLayers;
+        CommitLayers at{};
+        for (int l = 0; l < here; l++) {
+            at.kc[l] = kcaches[l0 + l];
+            at.vc[l] = vcaches[l0 + l];
+            at.kd[l] = kdrafts[l0 + l];
+            at.vd[l] = vdrafts[l0 + l];
+        }
+        cache_commit_kernel<<<dim3((unsigned)kv_heads, (unsigned)n, (unsigned)here), 256, 0, ctx->stream>>>(
+            at, M, max_nodes, first, path, counts, prefix, hd, context, draft_context, slots, nslots);
+        if (int rc = check_launch("commit of drafted entries"))
+            return rc;
+    }
+    return GX_OK;
+}
+
+int launch_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches, int kv_heads,
+                      int hd, int context, int src, const int32_t *dsts, int n, int len) {
+    for (int l0 = 0; l0 < layers; l0 += kCacheLayers)
+        for (int d0 = 0; d0 < n; d0 += kForkSlots) {
+            const int here = layers - l0 < kCacheLayers ? layers - l0 : kCacheLayers;
+            const int slots = n - d0 < kForkSlots ? n - d0 : kForkSlots;
+            ForkLayers at{};
+            for (int l = 0; l < here; l++) {
+                at.kc[l] = kcaches[l0 + l];
+                at.vc[l] = vcaches[l0 + l];
+            }
+            for (int d = 0; d < slots; d++)
+                at.dsts[d] = dsts[d0 + d];
+            cache_fork_kernel<<<dim3((unsigned)(kv_heads * hd / 8), 2, (unsigned)here), 256, 0, ctx->stream>>>(
+                at, kv_heads, hd, context, src, slots, len);
+            if (int rc = check_launch("fork of a conversation"))
+                return rc;
+        }
+    return GX_OK;
+}
+
+}  // namespace gx

@@ -201,6 +201,43 @@ int launch_qwen_swiglu_quant(gx_ctx *ctx, const float *gu, int ldgu, int M, int 
 int launch_argmax(gx_ctx *ctx, const float *x, int ldx, int M, int n, int32_t *out, int32_t *history,
                   int history_len, int32_t *pos, int32_t *positions, int32_t *row_tokens = nullptr,
                   int32_t *row_positions = nullptr);
+// Drafted trees (gx_tree.hip, gx_attn_tree.hip, gx_cache.hip).
+constexpr int kTreeNodes = 512;     // nodes a tree
+constexpr int kTrees = 1024;        // trees a call
+constexpr int kVocabMax = 1 << 20;  // tokens a row of logits that is drawn from
+constexpr int kForkSlots = 64;      // conversations a fork's one launch writes
+constexpr int kCacheLayers = 64;    // layers a cache copy's one launch takes
+struct TreeAttention {
+    const uint16_t *qh;
+    int n, M, max_nodes;
+    const int32_t *first;
+    const uint32_t *mask;
+    const int32_t *prefix;
+    int max_prefix, heads, kv_heads, hd;
+    const uint16_t *kcache, *vcache;
+    int context;
+    const uint16_t *kdraft, *vdraft;
+    int draft_context;
+    const int32_t *slots;
+    int nslots;
+};
+int launch_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *first, const int32_t *parents,
+                     const int32_t *prefix, const float *rope_cos, const float *rope_sin, int half, int context,
+                     int32_t *rows, int32_t *positions, uint32_t *mask, float *cos, float *sin);
+size_t attn_tree_workspace(int n, int M, int max_nodes, int heads, int kv_heads, int hd, int max_prefix);
+int launch_attn_tree(gx_ctx *ctx, const TreeAttention &y, float *out, int8_t *q, float *scales, int32_t *qsum,
+                     uint8_t *workspace);
+size_t tree_verify_workspace(int n, int M, int vocab);
+int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
+                       const int32_t *first, const int32_t *parents, const int32_t *tokens, const float *draft,
+                       int ldd, float temperature, float draft_temperature, const float *uniforms, int32_t *path,
+                       int32_t *counts, int32_t *next, uint8_t *workspace);
+int launch_cache_commit(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches,
+                        const uint16_t *const *kdrafts, const uint16_t *const *vdrafts, int n, int M, int max_nodes,
+                        const int32_t *first, const int32_t *path, const int32_t *counts, const int32_t *prefix,
+                        int kv_heads, int hd, int context, int draft_context, const int32_t *slots, int nslots);
+int launch_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches, int kv_heads,
+                      int hd, int context, int src, const int32_t *dsts, int n, int len);
 int launch_f32_matvec(gx_ctx *ctx, const gx_weight *w, const float *x, int ldx, int M, int row_start, int row_end,
                       float *y, int ldy);
 }  // namespace gx

@@ -581,6 +581,122 @@ int gx_argmax_step(gx_ctx *ctx, const float *x, int n, int32_t *ids, int32_t *hi
 int gx_argmax_slots_step(gx_ctx *ctx, const float *x, int ldx, int M, int n, int32_t *ids, int32_t *tokens,
                          int32_t *positions);
 
+/* ---- drafted tokens: trees over the Qwen3 caches ------------------------ */
+
+/* No counterpart in golem: a speculative step.  A pass runs n trees of drafted
+ * tokens through the model at once, one a conversation: token m of the batch
+ * (M in all) is node m - first[b] of tree b for first[b] <= m < first[b + 1]
+ * (first: n + 1 non-decreasing device int32 from 0; a tree of no nodes is
+ * allowed, tokens from first[n] on belong to none).  A tree has at most
+ * max_nodes nodes (max_nodes at most 512, n at most 1024, M at most 65535;
+ * nodes past max_nodes are treated as tokens of no tree).  Node 0 is the token
+ * the conversation has decided on and not yet run; parents[m] (device int32)
+ * is the node's parent within its tree, an earlier node, or -1 for a root.
+ * prefix[b] (device int32) counts the positions tree b's conversation has
+ * cached, and node i stands at position prefix[b] + its depth.
+ *
+ * The drafts' keys and values are not put into the caches but into draft
+ * buffers of the caches' layouts, token m at row m: kdraft
+ * [kv_heads][head_dim/8][draft_context][8], vdraft
+ * [kv_heads][head_dim][draft_context], draft_context a multiple of 8 of at
+ * least M.  So a layer of a pass is
+ *   gx_qwen_qkv_rope (or gx_qwen_qk_rope) with positions = the plan's rows,
+ *       rope_cos / rope_sin = the plan's, the draft buffers as caches, context
+ *       = draft_context and no slots;
+ *   gx_qwen_attention_tree
+ * and the layers' other calls as for any M positions; what the target rejects
+ * is forgotten, and gx_qwen_cache_commit puts the kept path into the caches. */
+
+/* What a pass's layers read, from the trees' parents: rows[m] = m, positions[m]
+ * = prefix[b] + depth, mask[m] (ceil(max_nodes/32) words) with bit j % 32 of
+ * word j / 32 set where node j is node m's ancestor or itself, and cos[m] /
+ * sin[m] = row positions[m] of rope_cos / rope_sin ([context][half] floats,
+ * half = head_dim / 2).  A node whose parent is neither an earlier node nor -1,
+ * every node below such a one, a node past `context`, and a token of no tree
+ * have no place: rows and positions -1, mask, cos and sin zero (gx_qwen_qk_rope
+ * then stores nothing and makes their query NaN).  All device pointers. */
+int gx_qwen_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *first, const int32_t *parents,
+                      const int32_t *prefix, const float *rope_cos, const float *rope_sin, int half, int context,
+                      int32_t *rows, int32_t *positions, uint32_t *mask, float *cos, float *sin);
+
+/* The attention of every node over what it sees: the first prefix[b] cached
+ * positions of its conversation and the nodes of its own tree whose bits its
+ * mask has (the plan's, or any others; bits past the tree's nodes are
+ * ignored), scores (1/sqrt(head_dim)) * query . key, softmax, values.  qh as
+ * gx_qwen_qk_rope writes it, the caches as gx_qwen_attention reads them
+ * (slots [n] / nslots: tree b's conversation, out of range clamped; NULL: one
+ * conversation's caches for every tree).  max_prefix bounds the prefixes; a
+ * larger one is cut to it, a negative one sees nothing cached.  Outputs, each
+ * optional but not both absent: out [M][heads*head_dim] floats, and the Q8_0
+ * form q/scales/qsum of the same values.  A node that sees nothing gives
+ * zeros; rows of tokens of no tree are left as they were; an infinite or NaN
+ * value reaches only the nodes that see it.  head_dim 32, 64, 96 or 128.
+ * qh, the caches and the draft buffers are 16-byte aligned.
+ *
+ * Float32 softmax statistics and sums in a fixed order; the probabilities
+ * enter the value products with about 22 bits (not golem's fp16 ones).  The
+ * order depends on n, max_nodes and max_prefix, so the last bits do; replays
+ * of a captured call give the bits of the eager one.  workspace: 256-byte
+ * aligned device memory of gx_qwen_attention_tree_workspace_bytes; calls that
+ * overlap need one each. */
+int gx_qwen_attention_tree_workspace_bytes(int n, int M, int max_nodes, int heads, int kv_heads, int head_dim,
+                                           int max_prefix, size_t *bytes);
+int gx_qwen_attention_tree(gx_ctx *ctx, const uint16_t *qh, int n, int M, int max_nodes, const int32_t *first,
+                           const uint32_t *mask, const int32_t *prefix, int max_prefix, int heads, int kv_heads,
+                           int head_dim, const uint16_t *kcache, const uint16_t *vcache, int context,
+                           const uint16_t *kdraft, const uint16_t *vdraft, int draft_context, float *out, int8_t *q,
+                           float *scales, int32_t *qsum, void *workspace, size_t workspace_bytes,
+                           const int32_t *slots, int nslots);
+
+/* Which drafted tokens the target agrees with.  logits [M][ldl] are the
+ * target's after each node, tokens [M] the nodes' tokens.  From node 0 the walk
+ * goes to a child of the node it is at until it takes none:
+ *   temperature 0: the first child whose token is the row's gx_argmax;
+ *   else with p = softmax(logits / temperature), the children in index order,
+ *   child m by its number uniforms[m] in [0, 1):
+ *     draft_logits NULL: drafts are given tokens.  Taken where u * N < p(token),
+ *       N what is left of p's mass, else p loses that token;
+ *     draft_logits [M][ldd]: drafts were drawn from q = softmax(draft_logits /
+ *       draft_temperature) of their parent's row, siblings without replacement.
+ *       Rejection sampling with the residual max(p - q, 0), renormalised child
+ *       after child.
+ * A child whose token an earlier sibling had, or that is outside the
+ * vocabulary, is passed over.  path [n][max_nodes] receives the nodes the walk
+ * went through (node 0 first, -1 behind them), counts [n] how many, next [n]
+ * the token after them: greedy the last row's argmax, else the least token at
+ * which the running sum of what is left of p passes uniforms[node 0] times its
+ * total (where rounding left nothing of p, p itself).  Kept tokens and the
+ * next are distributed as the target's own, whatever the drafts.  An empty
+ * tree gives count 0 and next -1; a row with a NaN or +inf logit, or none above
+ * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule).  Computed
+ * in float64.  uniforms may be NULL at temperature 0 only.  workspace as
+ * above; at temperature 0 the call also uses gx_argmax's scratch, with its
+ * rule.  vocab at most 2^20. */
+int gx_tree_verify_workspace_bytes(int n, int M, int vocab, size_t *bytes);
+int gx_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
+                   const int32_t *first, const int32_t *parents, const int32_t *tokens, const float *draft_logits,
+                   int ldd, float temperature, float draft_temperature, const float *uniforms, int32_t *path,
+                   int32_t *counts, int32_t *next, void *workspace, size_t workspace_bytes);
+
+/* The kept path's entries into the caches, all layers in one launch (64 layers
+ * a launch): node path[b][j] of tree b, j < counts[b], from its draft row to
+ * position prefix[b] + j of conversation slots[b] (NULL: conversation 0).  A
+ * node or position out of range, a negative prefix and a slot out of range
+ * store nothing.  kcaches, vcaches, kdrafts, vdrafts: host arrays of the
+ * layers' device pointers, read before the call returns.  Trees of one call
+ * belong to different conversations. */
+int gx_qwen_cache_commit(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches,
+                         const uint16_t *const *kdrafts, const uint16_t *const *vdrafts, int n, int M, int max_nodes,
+                         const int32_t *first, const int32_t *path, const int32_t *counts, const int32_t *prefix,
+                         int kv_heads, int head_dim, int context, int draft_context, const int32_t *slots,
+                         int nslots);
+
+/* Conversation src's positions 0 .. len - 1 into conversations dsts[0..n)
+ * (host ints, all different and not src), all layers; the rest of those
+ * conversations' caches stays.  kcaches, vcaches: host arrays as above. */
+int gx_qwen_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches, int nslots,
+                       int kv_heads, int head_dim, int context, int src, const int32_t *dsts, int n, int len);
+
 /* ---- calibration (measurement only) ----------------------------------- */
 
 /* No counterpart in golem; no product calls these.  They give the
