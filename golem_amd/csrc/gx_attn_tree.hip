@@ -258,8 +258,8 @@ __global__ __launch_bounds__(64) void attn_tree_join_kernel(const Args x, float 
     }
     const uint32_t *mrow = x.mask + (size_t)tok * x.words;
     bool any = t.P > 0;
-    for (int w = 0; w < x.words; w++)
-        any |= mrow[w] != 0;
+    for (int w = 0; 32 * w < t.T; w++)
+        any |= (mrow[w] & (t.T - 32 * w >= 32 ? ~0u : (1u << (t.T - 32 * w)) - 1)) != 0;
     if (any && l - l == 0.0f && o - o != 0.0f) {
         const int g = x.heads / x.kv_heads, kvh = head / g;
         const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;

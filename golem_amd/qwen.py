@@ -37,6 +37,13 @@ step's argmax and a device counter), and the attention is launched for the
 whole cache (max_pos = context - 1; the kernels stop at each position's own
 prefix), so every replay runs the same launches.  A replay computes exactly
 what the eager step computes.
+
+Drafted tokens run as trees, one a conversation, in one pass
+(forward_tree): gx_qwen_tree_plan, then the blocks with gx_qwen_qkv_rope
+storing into draft buffers and gx_qwen_attention_tree reading the caches and
+those.  verify_tree (gx_tree_verify) walks each tree by the target's logits and
+commit_tree (gx_qwen_cache_commit) puts the kept path into the caches;
+speculate is the loop over the three.
 """
 import ctypes
 import math
@@ -157,6 +164,8 @@ class QwenModel:
         self.history = torch.zeros((cfg.max_context + 1,), dtype=torch.int32, device="cuda")
         self.graph = None
         self.slot_graphs = {}
+        self.drafts = 0  # tokens the draft buffers hold (set_drafts)
+        self.tree_ws = None
         n = capi.size_out("gx_qwen_attention_workspace_bytes", M, cfg.heads, cfg.max_context - 1)
         self.attn_ws = torch.empty((n + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
         self._vp, self._call = vp, call
@@ -175,6 +184,7 @@ class QwenModel:
         self.kc = self.vc = None
         self.kc = [torch.zeros(kshape, dtype=torch.int16, device="cuda") for _ in range(cfg.layers)]
         self.vc = [torch.zeros(vshape, dtype=torch.int16, device="cuda") for _ in range(cfg.layers)]
+        self.tree = None  # a pass over drafted tokens read the caches being replaced
 
     def set_attention(self, attention):
         """Switch the decode steps' attention order ("parallel" or "golem");
@@ -558,6 +568,199 @@ class QwenModel:
         """The ids of `steps` greedy tokens from position `pos`: the seed
         and those the replays left in the history."""
         return [int(t) for t in self.history[pos:pos + steps].cpu().tolist()]
+
+    # ---- drafted tokens ----
+
+    def set_drafts(self, tokens):
+        """Draft buffers for passes of up to `tokens` drafted tokens, roots
+        included (at most max_batch): a layer's keys and values in the caches'
+        layouts, a token a row."""
+        cfg, dev = self.cfg, "cuda"
+        if not 0 < tokens <= self.max_batch:
+            raise ValueError(f"qwen: {tokens} drafted tokens for a batch of {self.max_batch}")
+        self.drafts, self.tree = tokens, None
+        self.draft_context = (tokens + 7) // 8 * 8
+        kshape = (cfg.kv_heads, cfg.head_dim // 8, self.draft_context, 8)
+        vshape = (cfg.kv_heads, cfg.head_dim, self.draft_context)
+        self.kd = [torch.zeros(kshape, dtype=torch.int16, device=dev) for _ in range(cfg.layers)]
+        self.vd = [torch.zeros(vshape, dtype=torch.int16, device=dev) for _ in range(cfg.layers)]
+        half = cfg.head_dim // 2
+        self.draft_cos = torch.empty((tokens, half), dtype=torch.float32, device=dev)
+        self.draft_sin = torch.empty((tokens, half), dtype=torch.float32, device=dev)
+        self.draft_rows = torch.empty((tokens,), dtype=torch.int32, device=dev)
+
+    def _tree_workspace(self, name, *size):
+        n = (capi.size_out(name, *size) + 255) // 256 * 256
+        if self.tree_ws is None or self.tree_ws.numel() < n:
+            self.tree_ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        return self._vp(self.tree_ws), self.tree_ws.numel()
+
+    def forward_tree(self, tokens, parents, prefixes, slots=None):
+        """One pass over a tree of drafted tokens for each of several
+        conversations.  tokens[b] and parents[b] list tree b's nodes: node 0
+        is the token decided on and not yet run (parent -1), every other
+        node's parent an earlier one.  prefixes[b] counts the positions
+        conversation slots[b] (default: the current slot, for one tree) has
+        cached.  Returns the device hidden states [M][dim] after the final
+        norm, the trees' nodes one after another; the caches stay as they are
+        until commit_tree."""
+        n, sizes = len(tokens), [len(t) for t in tokens]
+        slots = [self.slot] * n if slots is None else list(slots)
+        M, nodes = sum(sizes), max(sizes, default=0)
+        if not len(parents) == len(prefixes) == len(slots) == n or n == 0 or min(sizes) == 0:
+            raise ValueError("qwen: a tree needs tokens, parents, a prefix and a slot")
+        if M > self.drafts:
+            raise ValueError(f"qwen: {M} drafted tokens for buffers of {self.drafts} (set_drafts)")
+        if len(set(slots)) != n:
+            raise ValueError("qwen: two trees of one conversation")
+        for t, p, prefix, slot in zip(tokens, parents, prefixes, slots):
+            if not 0 <= slot < self.nslots:
+                raise IndexError(f"qwen: slot {slot} of {self.nslots}")
+            depth = []
+            for i, up in enumerate(p):
+                if len(p) != len(t) or not (up == -1 if i == 0 else 0 <= up < i):
+                    raise ValueError(f"qwen: node {i}'s parent {up} is no earlier node")
+                depth.append(0 if i == 0 else depth[up] + 1)
+            if prefix < 0 or prefix + max(depth) >= self.slot_context:
+                raise ValueError(f"qwen: position {prefix + max(depth)} is past the context {self.slot_context}")
+
+        def dev(v):
+            return torch.tensor(np.asarray(v, dtype=np.int32), device="cuda")
+
+        def flat(v):
+            return [x for row in v for x in row]
+
+        first = np.concatenate([[0], np.cumsum(sizes)])
+        self.tokens[:M].copy_(dev(flat(tokens)))
+        self.tree = {"n": n, "M": M, "nodes": nodes, "first": dev(first), "parents": dev(flat(parents)),
+                     "prefix": dev(prefixes), "slots": dev(slots), "max_prefix": int(max(prefixes)),
+                     "mask": torch.empty((M, (nodes + 31) // 32), dtype=torch.int32, device="cuda"),
+                     "path": torch.empty((n, nodes), dtype=torch.int32, device="cuda"),
+                     "counts": torch.empty((n,), dtype=torch.int32, device="cuda"),
+                     "next": torch.empty((n,), dtype=torch.int32, device="cuda")}
+        self._tree_blocks(self.tree)
+        return self.hidden[:M]
+
+    def _tree_blocks(self, t):
+        """The embedding rows, blocks and final norm of forward_tree, from the
+        device state alone (so that it can be captured, the workspace being
+        there)."""
+        cfg, vp, call, ctx = self.cfg, self._vp, self._call, self.ctx.ptr
+        n, M, nodes, qd = t["n"], t["M"], t["nodes"], self.qd
+        eps = np.float32(cfg.eps)
+        call("gx_qwen_tree_plan", ctx, n, M, nodes, vp(t["first"]), vp(t["parents"]), vp(t["prefix"]),
+             vp(self.rope_cos), vp(self.rope_sin), cfg.head_dim // 2, self.slot_context, vp(self.draft_rows),
+             vp(self.positions), vp(t["mask"]), vp(self.draft_cos), vp(self.draft_sin))
+        call("gx_weight_rows", ctx, self.embd.ptr, 0, vp(self.tokens), M, vp(self.xs))
+        ws, size = self._tree_workspace("gx_qwen_attention_tree_workspace_bytes", n, M, nodes, cfg.heads,
+                                        cfg.kv_heads, cfg.head_dim, t["max_prefix"])
+        for i, b in enumerate(self.blocks):
+            call("gx_norm_quant", ctx, vp(self.xs), cfg.dim, None if i == 0 else vp(self.ffn), cfg.dim,
+                 vp(b["attn_norm"]), M, cfg.dim, eps, None, 0, vp(self.x8.q), vp(self.x8.s), vp(self.x8.qs))
+            # the drafts' own buffers as caches, the plan's rows as positions
+            call("gx_qwen_qkv_rope", ctx, b["qkv"].ptr, vp(self.x8.q), vp(self.x8.s), vp(self.x8.qs), M,
+                 cfg.heads, cfg.kv_heads, cfg.head_dim, vp(self.draft_rows), vp(b["q_norm"]), vp(b["k_norm"]),
+                 vp(self.draft_cos), vp(self.draft_sin), eps, vp(self.qh), vp(self.kd[i]), vp(self.vd[i]),
+                 self.draft_context, None, 0, vp(self.qkv))
+            call("gx_qwen_attention_tree", ctx, vp(self.qh), n, M, nodes, vp(t["first"]), vp(t["mask"]),
+                 vp(t["prefix"]), t["max_prefix"], cfg.heads, cfg.kv_heads, cfg.head_dim, vp(self.kc[i]),
+                 vp(self.vc[i]), self.context, vp(self.kd[i]), vp(self.vd[i]), self.draft_context, None,
+                 vp(self.set8.q), vp(self.set8.s), vp(self.set8.qs), ws, size, vp(t["slots"]), self.nslots)
+            self._mm(b["o"], self.set8, M, self.attn, cfg.dim)
+            call("gx_norm_quant", ctx, vp(self.xs), cfg.dim, vp(self.attn), cfg.dim, vp(b["ffn_norm"]), M, cfg.dim,
+                 eps, None, 0, vp(self.x8.q), vp(self.x8.s), vp(self.x8.qs))
+            call("gx_matmul_swiglu_q4_0", ctx, b["gu"].ptr, vp(self.x8.q), vp(self.x8.s), vp(self.x8.qs), M,
+                 vp(self.mid8.q), vp(self.mid8.s), vp(self.mid8.qs))
+            self._mm(b["down"], self.mid8, M, self.ffn, cfg.dim)
+        call("gx_norm_quant", ctx, vp(self.xs), cfg.dim, vp(self.ffn), cfg.dim, vp(self.output_norm), M, cfg.dim,
+             eps, vp(self.hidden), cfg.dim, None, None, None)
+
+    def verify_tree(self, temperature=0.0, draft_logits=None, draft_temperature=None, uniforms=None):
+        """The walk down the trees of the last forward_tree by the target's
+        logits (gx_tree_verify): temperature 0 keeps the drafts that greedy
+        decoding would have drawn; above, each node's number in `uniforms`
+        (device float32 [M], in [0, 1); default: torch's generator) decides,
+        the drafts being given tokens or, with draft_logits (device [M][vocab],
+        the draft model's logits after each node), drawn from their softmax at
+        draft_temperature (default: temperature).  Returns device tensors:
+        path [trees][nodes] (-1 behind), counts [trees], next [trees]."""
+        t, vp, V = self._a_tree(), self._vp, self.cfg.vocab
+        M = t["M"]
+        if uniforms is None and temperature > 0:
+            uniforms = torch.rand((M,), device="cuda")
+        for x, shape, what in ((draft_logits, (M, V), "draft logits"), (uniforms, (M,), "random numbers")):
+            if x is not None and not (tuple(x.shape) == shape and x.dtype == torch.float32 and x.is_cuda
+                                      and x.is_contiguous()):
+                raise ValueError(f"qwen: the {what} are a contiguous float32 {shape} on the GPU, not "
+                                 f"{x.dtype} {tuple(x.shape)} on {x.device}")
+        logits = self.logits_batch(range(M))
+        ws, size = self._tree_workspace("gx_tree_verify_workspace_bytes", t["n"], M, V)
+        self._call("gx_tree_verify", self.ctx.ptr, vp(logits), V, t["n"], M, t["nodes"], V, vp(t["first"]),
+                   vp(t["parents"]), vp(self.tokens), vp(draft_logits), V, temperature,
+                   temperature if draft_temperature is None else draft_temperature, vp(uniforms), vp(t["path"]),
+                   vp(t["counts"]), vp(t["next"]), ws, size)
+        return t["path"], t["counts"], t["next"]
+
+    def commit_tree(self):
+        """The kept paths of the last verify_tree into their conversations'
+        caches: prefixes[b] + counts[b] positions are cached then."""
+        t, vp, cfg = self._a_tree(), self._vp, self.cfg
+        layers = [(ctypes.c_void_p * cfg.layers)(*[x.data_ptr() for x in xs])
+                  for xs in (self.kc, self.vc, self.kd, self.vd)]
+        self._call("gx_qwen_cache_commit", self.ctx.ptr, cfg.layers, *layers, t["n"], t["M"], t["nodes"],
+                   vp(t["first"]), vp(t["path"]), vp(t["counts"]), vp(t["prefix"]), cfg.kv_heads, cfg.head_dim,
+                   self.context, self.draft_context, vp(t["slots"]), self.nslots)
+
+    def _a_tree(self):
+        if self.tree is None:
+            raise ValueError("qwen: no pass over drafted tokens (forward_tree)")
+        return self.tree
+
+    def fork_slot(self, src, dsts, length):
+        """The first `length` positions of conversation src into each of dsts:
+        conversations with a common beginning read it once."""
+        cfg, dsts = self.cfg, list(dsts)
+        if not 0 <= length <= self.slot_context:
+            raise ValueError(f"qwen: {length} positions of a slot's {self.slot_context}")
+        layers = [(ctypes.c_void_p * cfg.layers)(*[x.data_ptr() for x in xs]) for xs in (self.kc, self.vc)]
+        self._call("gx_qwen_cache_fork", self.ctx.ptr, cfg.layers, *layers, self.nslots, cfg.kv_heads, cfg.head_dim,
+                   self.context, src, (ctypes.c_int32 * len(dsts))(*dsts), len(dsts), length)
+
+    def speculate(self, prompt, steps, draft, temperature=0.0, generator=None):
+        """`steps` tokens after the prompt, several a pass where drafts are
+        kept.  draft(ids) proposes a tree after the ids so far: (tokens,
+        parents) of nodes 1, 2, .., parents as node numbers with 0 the last
+        id, or with a third entry, the device draft logits [1 + nodes][vocab]
+        that the tokens were drawn from.  temperature 0: greedy's tokens;
+        above, random numbers come from `generator` (a torch generator of the
+        GPU).  Returns the ids and the number of passes."""
+        if not prompt or len(prompt) + steps - 1 > self.slot_context:
+            raise ValueError(f"qwen: {steps} tokens after {len(prompt)} exceed the context {self.slot_context}")
+        if self.drafts == 0:
+            self.set_drafts(self.max_batch)
+        ids, passes, cached = [int(x) for x in prompt], 0, len(prompt) - 1
+        for at in range(0, cached, self.max_batch):
+            self.forward(ids[at:min(cached, at + self.max_batch)], at)
+        while len(ids) < len(prompt) + steps:
+            tokens, parents, *logits = draft(list(ids))
+            depth, keep = [0], 1  # nodes within the context, the buffers and the steps asked for
+            for p in parents[:self.drafts - 1]:
+                depth.append(depth[p] + 1)
+                if cached + depth[-1] >= self.slot_context:
+                    break
+                keep += 1
+            tree = [ids[-1]] + [int(x) for x in tokens[:keep - 1]]
+            self.forward_tree([tree], [[-1] + list(parents[:keep - 1])], [cached])
+            uniforms = None if temperature == 0 else torch.rand((keep,), generator=generator, device="cuda")
+            path, counts, nxt = self.verify_tree(temperature, logits[0][:keep] if logits else None,
+                                                 uniforms=uniforms)
+            self.commit_tree()
+            count = int(counts[0])
+            kept = path[0, :count].tolist()
+            ids += [tree[i] for i in kept[1:]] + [int(nxt[0])]
+            cached += count
+            passes += 1
+        return ids[len(prompt):len(prompt) + steps], passes
 
     def free(self):
         for b in self.blocks:

@@ -630,7 +630,9 @@ int gx_qwen_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *f
  * optional but not both absent: out [M][heads*head_dim] floats, and the Q8_0
  * form q/scales/qsum of the same values.  A node that sees nothing gives
  * zeros; rows of tokens of no tree are left as they were; an infinite or NaN
- * value reaches only the nodes that see it.  head_dim 32, 64, 96 or 128.
+ * value reaches only the nodes that see it (an element beside a hidden one is
+ * summed again in another order: its last bits may differ).  head_dim 32, 64,
+ * 96 or 128.
  * qh, the caches and the draft buffers are 16-byte aligned.
  *
  * Float32 softmax statistics and sums in a fixed order; the probabilities
@@ -668,8 +670,9 @@ int gx_qwen_attention_tree(gx_ctx *ctx, const uint16_t *qh, int n, int M, int ma
  * total (where rounding left nothing of p, p itself).  Kept tokens and the
  * next are distributed as the target's own, whatever the drafts.  An empty
  * tree gives count 0 and next -1; a row with a NaN or +inf logit, or none above
- * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule).  Computed
- * in float64.  uniforms may be NULL at temperature 0 only.  workspace as
+ * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule), and so
+ * does a node with children whose draft row has a NaN or +inf.  Computed in
+ * float64.  uniforms may be NULL at temperature 0 only.  workspace as
  * above; at temperature 0 the call also uses gx_argmax's scratch, with its
  * rule.  vocab at most 2^20. */
 int gx_tree_verify_workspace_bytes(int n, int M, int vocab, size_t *bytes);
