@@ -115,29 +115,40 @@ __global__ __launch_bounds__(kPlanThreads) void tree_plan_kernel(
 
 constexpr int kStatThreads = 256;
 constexpr int kStatChunk = 8192;  // tokens a workgroup of the row sums takes
-constexpr int kWalkThreads = 1024;
-constexpr int kPickChunk = 2048;  // tokens a running sum is kept for
+constexpr int kWalkThreads = 256;
+constexpr int kPart = 2048;       // tokens a part of a running sum, eight a thread
+constexpr int kParts = kVocabMax / kPart;
+constexpr int kWalkGroups = 512;  // workgroups of a walk, over all its trees
 
-struct RowStat {
-    double top, sum;  // the row's largest logit, the sum of e^((l - top) / T)
+// e^((x - top) / T) as 2^(y / 32), y = (x - top) 32 / (T ln 2): n = rint(y),
+// e^((y - n) ln 2 / 32) by its Taylor series to the fifth power (the argument
+// within 0.011: 3e-15 off) times 2^(n mod 32 / 32) from a table in LDS (32
+// entries, each on banks of its own) and 2^(n div 32).  A chance below 2^-1000
+// is none, and so is that of -inf; a NaN stays one.
+struct Exp64 {
+    double A, top;
+    const double *table;
+    __device__ Exp64(const double *lds, double inv, double t)
+        : A(inv * 0x1.71547652b82fep+5), top(t == -INFINITY ? 0.0 : t), table(lds) {}
+    __device__ __forceinline__ double operator()(float x) const {
+        const double y = ((double)x - top) * A;
+        const double n = __builtin_rint(y), f = y - n;
+        double p = 0x1.5d87fe78a6730p-35;  // ln2^5 / 120 / 32^5, and so down
+        p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-27);
+        p = __builtin_fma(p, f, 0x1.c6b08d704a0bfp-20);
+        p = __builtin_fma(p, f, 0x1.ebfbdff82c58ep-13);
+        p = __builtin_fma(p, f, 0x1.62e42fefa39efp-6);
+        p = p * f;
+        const int ni = (int)n;
+        const double t = table[ni & 31];
+        const double e = __builtin_ldexp(__builtin_fma(t, p, t), ni >> 5);
+        return y < -32000.0 ? 0.0 : e;
+    }
 };
 
-// e^d for d <= 0: exp_neg's steps, the float64 left as it is (within an ulp).
-__device__ __forceinline__ double exp64(double d) {
-    const double n = __builtin_rint(d * 0x1.71547652b82fep+6);
-    double r = __builtin_fma(-n, 0x1.62e42fefa38p-7, d);
-    r = __builtin_fma(-n, 0x1.ef358p-51, r);
-    double p = 1.0 / 720.0;
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = p * r;
-    const int ni = (int)n;
-    const double t = kExp2Sixtyfourths[ni & 63];
-    const double out = __builtin_ldexp(__builtin_fma(t, p, t), ni >> 6);
-    return d < -740.0 ? 0.0 : out;
+__device__ __forceinline__ void exp64_table(double *lds) {
+    if (threadIdx.x < 32)
+        lds[threadIdx.x] = kExp2Sixtyfourths[2 * threadIdx.x];
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -146,21 +157,45 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
+// What a walk's workgroups share, one a tree.  The first of them walks; where
+// it needs a sum over a row it hands out the row's parts to whoever asks, the
+// others and itself, and waits for the parts that were taken: only ever for a
+// workgroup that runs.  The others wait only for one that walks: a workgroup
+// that finds none walking after a while ends, and so do all when the walk does.
+struct Share {
+    unsigned long long claim;  // the sum's number in the high half, the next part in the low
+    unsigned fin;              // parts that are summed
+    unsigned walking, done;
+    int row, turned;
+    double top, scale, dtop, dscale;  // what is left of token x: scale e^((l_x - top) / T) - dscale e^(..)
+    double part[kParts];
+    int gone[kTreeNodes];
+};
+
+template <typename T>
+__device__ __forceinline__ T share_load(const T *p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ void share_store(T *p, T v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // grid (chunks, M, 1 or 2): a chunk's largest logit and sum of exponentials,
-// of the target's rows (z 0) and the draft's.  A logit of -inf has no chance;
-// a NaN or +inf makes the sum NaN.
+// of the target's rows (z 0) and the draft's; and the walks' shares cleared.
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float *__restrict__ logits, int ldl,
                                                                     const float *__restrict__ draft, int ldd,
                                                                     int vocab, double it, double itd,
                                                                     float *__restrict__ tops,
-                                                                    double *__restrict__ sums) {
+                                                                    double *__restrict__ sums, Share *share, int n) {
     constexpr int kMine = kStatChunk / kStatThreads;
     __shared__ float wt[kStatThreads / 64];
     __shared__ double wsum[kStatThreads / 64];
+    __shared__ double table[32];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.y, c0 = blockIdx.x * kStatChunk;
     const float *x = blockIdx.z ? draft + (size_t)row * ldd : logits + (size_t)row * ldl;
-    const double inv = blockIdx.z ? itd : it;
+    exp64_table(table);
     float v[kMine];
     float top = -INFINITY;
 #pragma unroll
@@ -177,11 +212,11 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
     __syncthreads();
     for (int w = 0; w < kStatThreads / 64; w++)
         top = fmaxf(top, wt[w]);
+    const Exp64 e(table, blockIdx.z ? itd : it, top);
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kMine; k++)
-        if (v[k] != -INFINITY)
-            sum += exp64(((double)v[k] - (double)top) * inv);
+        sum += e(v[k]);
     sum = wave_sum64(sum);
     if (lane == 0)
         wsum[wave] = sum;
@@ -193,49 +228,151 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
         tops[at] = top;
         sums[at] = sum;
     }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
+        for (int b = tid; b < n; b += kStatThreads) {
+            share[b].claim = 0;
+            share[b].walking = share[b].done = 0;
+        }
 }
 
 struct WalkArgs {
     const float *logits, *draft, *uniforms;
-    int ldl, ldd, M, max_nodes, vocab, chunks;
+    int ldl, ldd, M, max_nodes, vocab, chunks, groups;
     const int32_t *first, *parents, *tokens, *picks;
     double it, itd;
     const float *tops;
     const double *sums;
+    Share *share;
     int32_t *path, *counts, *next;
 };
 
-// A row's statistics from its chunks' (every lane of the wavefront).
-__device__ __forceinline__ RowStat row_stat(const float *tops, const double *sums, int chunks, double inv) {
-    const int lane = threadIdx.x & 63;
-    float top = -INFINITY;
-    for (int i = lane; i < chunks; i += 64)
-        top = fmaxf(top, tops[i]);
-    top = wave_max(top);
-    double sum = 0.0;
-    for (int i = lane; i < chunks; i += 64)
-        if (sums[i] != 0.0)  // (a chunk without a chance has no largest logit either)
-            sum += sums[i] * exp64(((double)tops[i] - (double)top) * inv);
-    return {(double)top, wave_sum64(sum)};
+// The chance left to a token of a row, from both rows' logits.
+struct Left {
+    const float *lr, *dr;  // dr NULL: nothing of the draft's to take off
+    Exp64 p, q;
+    double scale, dscale;
+    const int *gone;
+    int turned;
+    __device__ double operator()(int x) const {
+        double r = p(lr[x]) * scale;
+        if (dr) {
+            r -= q(dr[x]) * dscale;
+            return r < 0.0 ? 0.0 : r;
+        }
+        for (int i = 0; i < turned; i++)
+            if (gone[i] == x)
+                r = 0.0;
+        return r;
+    }
+};
+
+// One part's sum, by the whole workgroup (every thread gets it): eight tokens
+// a thread, a wavefront's 64 tokens in a row.
+__device__ __forceinline__ double part_sum(const Left &left, int k, int vocab, double *wsum) {
+    const int tid = threadIdx.x, x0 = k * kPart + tid;
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPart / kWalkThreads; i++)
+        if (x0 + i * kWalkThreads < vocab)
+            s += left(x0 + i * kWalkThreads);
+    s = wave_sum64(s);
+    __syncthreads();
+    if ((tid & 63) == 0)
+        wsum[tid >> 6] = s;
+    __syncthreads();
+    s = wsum[0];
+    for (int w = 1; w < kWalkThreads / 64; w++)
+        s += wsum[w];
+    return s;
 }
 
-// grid n: a workgroup a tree.
+// One part of the sum that is open, workgroup-wide; false where the claim came
+// after the last.
+struct Helper {
+    const WalkArgs &a;
+    Share &sh;
+    const double *table;
+    double *wsum;
+    int *gone;
+    int parts;
+    __device__ bool one(unsigned long long old) {  // old: a claim of this workgroup, the same in every thread
+        const int k = (int)(unsigned)old;
+        if (k >= parts)
+            return false;
+        const int row = share_load(&sh.row), turned = share_load(&sh.turned);
+        const double dscale = share_load(&sh.dscale);
+        const Left left{a.logits + (size_t)row * a.ldl,
+                        dscale > 0.0 ? a.draft + (size_t)row * a.ldd : nullptr,
+                        Exp64(table, a.it, share_load(&sh.top)),
+                        Exp64(table, a.itd, share_load(&sh.dtop)),
+                        share_load(&sh.scale),
+                        dscale,
+                        gone,
+                        a.draft ? 0 : turned};
+        if (!a.draft) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < turned; i += kWalkThreads)
+                gone[i] = share_load(&sh.gone[i]);
+            __syncthreads();
+        }
+        const double s = part_sum(left, k, a.vocab, wsum);
+        if (threadIdx.x == 0) {
+            share_store(&sh.part[k], s);
+            __hip_atomic_fetch_add(&sh.fin, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        return true;
+    }
+};
+
+constexpr int kPolls = 400;  // looks for a walk that has begun, before a helper ends
+
+// grid (groups, n): a tree's first workgroup walks, the others help.
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArgs a) {
-    __shared__ int par[kTreeNodes], tok[kTreeNodes];
-    __shared__ double part[kWalkThreads / 64];
-    __shared__ double run[kVocabMax / kPickChunk];
-    __shared__ int gone[kTreeNodes];  // the tokens turned down at this node
+    __shared__ int par[kTreeNodes], tok[kTreeNodes], gone[kTreeNodes];
+    __shared__ double px[kTreeNodes], qx[kTreeNodes];                        // a node's token by its parent's rows
+    __shared__ double top[kTreeNodes], sum[kTreeNodes], dtop[kTreeNodes], dsum[kTreeNodes];  // a node's own rows
+    __shared__ double run[kParts], table[32], wsum[kWalkThreads / 64];
+    __shared__ unsigned long long got;
     __shared__ int found;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y;
     const int f0 = min(max(a.first[b], 0), a.M), T = min(min(max(a.first[b + 1], f0), a.M) - f0, a.max_nodes);
+    const int parts = (a.vocab + kPart - 1) / kPart;
+    Share &sh = a.share[b];
+    Helper help{a, sh, table, wsum, gone, parts};
+    if (blockIdx.x > 0) {
+        if (T <= 0)
+            return;
+        exp64_table(table);
+        unsigned spent = 0;
+        for (;;) {
+            __syncthreads();
+            if (tid == 0) {
+                unsigned long long c = ~0ull;  // nothing more comes
+                for (;;) {
+                    if (share_load(&sh.done))
+                        break;
+                    if (!share_load(&sh.walking) && ++spent > kPolls)
+                        break;
+                    c = share_load(&sh.claim);
+                    if (c >> 32 && (unsigned)c < (unsigned)parts) {
+                        c = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
+                        break;
+                    }
+                    c = ~0ull;
+                    __builtin_amdgcn_s_sleep(4);
+                }
+                got = c;
+            }
+            __syncthreads();
+            const unsigned long long mine = got;
+            if (mine == ~0ull)
+                return;
+            help.one(mine);
+        }
+    }
     int32_t *path = a.path + (size_t)b * a.max_nodes;
     for (int i = tid; i < a.max_nodes; i += kWalkThreads)
         path[i] = -1;
-    for (int i = tid; i < T; i += kWalkThreads) {
-        par[i] = a.parents[f0 + i];
-        tok[i] = a.tokens[f0 + i];
-    }
-    __syncthreads();
     if (T <= 0) {
         if (tid == 0) {
             a.counts[b] = 0;
@@ -243,6 +380,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         return;
     }
+    if (tid == 0 && !a.picks)
+        share_store(&sh.walking, 1u);
+    exp64_table(table);
+    for (int i = tid; i < T; i += kWalkThreads) {
+        par[i] = a.parents[f0 + i];
+        tok[i] = a.tokens[f0 + i];
+    }
+    __syncthreads();  // (and the path's -1s are written)
     if (tid == 0)
         path[0] = 0;
     int v = 0, kept = 1;
@@ -260,107 +405,143 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         return;
     }
-    const float *lr = nullptr, *dr = nullptr;
-    RowStat st{}, sd{};
+    // every row's statistics from its chunks', then every child's chances
+    for (int i = tid; i < T * 2; i += kWalkThreads) {
+        const int node = i >> 1, z = i & 1;
+        if (z && !a.draft)
+            continue;
+        const size_t at = ((size_t)z * a.M + f0 + node) * a.chunks;
+        float mx = -INFINITY;
+        for (int c = 0; c < a.chunks; c++)
+            mx = fmaxf(mx, a.tops[at + c]);
+        const Exp64 e(table, z ? a.itd : a.it, mx);
+        double s = 0.0;
+        for (int c = 0; c < a.chunks; c++)
+            if (a.sums[at + c] != 0.0)
+                s += a.tops[at + c] == -INFINITY ? a.sums[at + c] : a.sums[at + c] * e(a.tops[at + c]);
+        (z ? dtop : top)[node] = mx;
+        (z ? dsum : sum)[node] = s;
+    }
+    __syncthreads();
+    for (int m = tid; m < T; m += kWalkThreads) {
+        const int p = par[m], x = tok[m];
+        if (p < 0 || p >= m || x < 0 || x >= a.vocab)
+            continue;
+        px[m] = Exp64(table, a.it, top[p])(a.logits[(size_t)(f0 + p) * a.ldl + x]) / sum[p];
+        if (a.draft)
+            qx[m] = Exp64(table, a.itd, dtop[p])(a.draft[(size_t)(f0 + p) * a.ldd + x]) / dsum[p];
+    }
+    __syncthreads();
     double c = 0.0, tried = 0.0, mass = 1.0;
     int turned = 0;
-    auto enter = [&]() {
-        const size_t row = f0 + v;
-        lr = a.logits + row * a.ldl;
-        st = row_stat(a.tops + row * a.chunks, a.sums + row * a.chunks, a.chunks, a.it);
-        if (a.draft) {
-            dr = a.draft + row * a.ldd;
-            sd = row_stat(a.tops + (a.M + row) * a.chunks, a.sums + (a.M + row) * a.chunks, a.chunks, a.itd);
-        }
-        c = tried = 0.0;
-        mass = 1.0;
-        turned = 0;
+    unsigned sums = 0;
+    bool known = true;   // mass is up to date
+    bool summed = false; // run[] holds the parts of what is left
+    // the factor of the draft's exponentials in what is left (a row of q that is
+    // none takes nothing off)
+    auto off = [&]() {
+        const double d = a.draft ? c / dsum[v] : 0.0;
+        return d > 0.0 && d - d == 0.0 ? d : 0.0;
     };
-    auto pt = [&](int x) { return lr[x] == -INFINITY ? 0.0 : exp64(((double)lr[x] - st.top) * a.it) / st.sum; };
-    auto qd = [&](int x) { return dr[x] == -INFINITY ? 0.0 : exp64(((double)dr[x] - sd.top) * a.itd) / sd.sum; };
-    auto was = [&](int x) {
-        for (int i = 0; i < turned; i++)
-            if (gone[i] == x)
-                return true;
-        return false;
-    };
-    // what is left of token x's chance
-    auto left = [&](int x) {
-        const double p = pt(x);
-        if (a.draft) {
-            const double r = c > 0.0 ? p - c * qd(x) : p;
-            return r < 0.0 ? 0.0 : r;
-        }
-        return was(x) ? 0.0 : p;
-    };
-    // the sum of left() in chunks of kPickChunk, a wavefront a chunk, then in order
-    const int parts = (a.vocab + kPickChunk - 1) / kPickChunk;
+    // the sum of what is left of v's row
     auto total = [&]() {
-        __syncthreads();
-        for (int k = wave; k < parts; k += kWalkThreads / 64) {
-            double s = 0.0;
-            for (int i = lane; i < kPickChunk; i += 64)
-                if (k * kPickChunk + i < a.vocab)
-                    s += left(k * kPickChunk + i);
-            s = wave_sum64(s);
-            if (lane == 0)
-                run[k] = s;
+        if (tid == 0) {
+            share_store(&sh.row, f0 + v);
+            share_store(&sh.turned, turned);
+            share_store(&sh.top, top[v]);
+            share_store(&sh.scale, 1.0 / sum[v]);
+            share_store(&sh.dtop, a.draft ? dtop[v] : 0.0);
+            share_store(&sh.dscale, off());
+            for (int i = 0; i < turned; i++)
+                share_store(&sh.gone[i], gone[i]);
+            share_store(&sh.fin, 0u);
+            __hip_atomic_store(&sh.claim, (unsigned long long)++sums << 32, __ATOMIC_RELEASE,
+                               __HIP_MEMORY_SCOPE_AGENT);
         }
+        for (;;) {
+            __syncthreads();
+            if (tid == 0)
+                got = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (!help.one(got))
+                break;
+        }
+        if (tid == 0)
+            while (__hip_atomic_load(&sh.fin, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) < (unsigned)parts)
+                __builtin_amdgcn_s_sleep(1);
+        __syncthreads();
+        for (int k = tid; k < parts; k += kWalkThreads)
+            run[k] = share_load(&sh.part[k]);
         __syncthreads();
         double s = 0.0;
         for (int k = 0; k < parts; k++)
             s += run[k];
+        summed = true;
         return s;
     };
-    enter();
     for (int m = 1; m < T; m++) {
         if (par[m] != v)
             continue;
         const int x = tok[m];
-        if (x < 0 || x >= a.vocab || was(x))
-            continue;  // no token, or one turned down already: passed over
+        bool over = x < 0 || x >= a.vocab;  // no token, or one turned down already: passed over
+        for (int i = 0; i < turned; i++)
+            over |= gone[i] == x;
+        if (over)
+            continue;
         const double u = (double)a.uniforms[f0 + m];
         bool take;
-        const double px = left(x);
         if (a.draft) {
-            const double rest = 1.0 - tried, qx = qd(x);
+            const double rest = 1.0 - tried;
+            if (!known)
+                mass = total();
+            known = true;
             if (!(rest > 0.0) || !(mass > 0.0))
                 continue;  // nothing a draft could have come from is left
-            take = u * mass * qx < px * rest;
+            const double r = px[m] - c * qx[m];
+            take = u * mass * qx[m] < (r < 0.0 ? 0.0 : r) * rest;
             if (!take) {
                 c += mass / rest;
-                tried += qx;
-                mass = total();
+                tried += qx[m];
+                known = summed = false;
             }
         } else {
-            take = u * mass < px;
+            take = u * mass < px[m];
             if (!take)
-                mass -= px;
+                mass -= px[m];
         }
+        __syncthreads();
         if (take) {
             if (tid == 0)
                 path[kept] = m;
             v = m;
             kept++;
-            __syncthreads();
-            enter();
+            c = tried = 0.0;
+            mass = 1.0;
+            turned = 0;
+            known = true;
+            summed = false;
         } else {
-            __syncthreads();
             if (tid == 0)
                 gone[turned] = x;
             turned++;
-            __syncthreads();
         }
+        __syncthreads();
     }
-    double sum = total();
-    if (!(sum > 0.0) && sum == 0.0) {  // rounding left nothing: the row as it was
+    double all = 0.0;
+    for (int k = 0; summed && k < parts; k++)
+        all += run[k];
+    if (!summed)
+        all = total();
+    if (all == 0.0 && (c > 0.0 || turned > 0)) {  // rounding left nothing: the row as it was
         c = 0.0;
         turned = 0;
-        sum = total();
+        all = total();
     }
+    if (tid == 0)
+        share_store(&sh.done, 1u);
     int token = -1;
-    if (sum > 0.0 && sum - sum == 0.0) {
-        const double aim = (double)a.uniforms[f0] * sum;
+    if (all > 0.0 && all - all == 0.0) {
+        const double aim = (double)a.uniforms[f0] * all;
         double s = 0.0;
         int k = 0, last = 0;
         for (int i = 0; i < parts; i++)
@@ -368,45 +549,60 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 last = i;
         for (; k < last && s + run[k] <= aim; k++)
             s += run[k];
-        // within the chunk, 1,024 tokens a round: a running sum over the wavefronts
+        // the part's running sum: eight tokens in a row a thread
+        constexpr int kEach = kPart / kWalkThreads;
+        const Left left{a.logits + (size_t)(f0 + v) * a.ldl,
+                        off() > 0.0 ? a.draft + (size_t)(f0 + v) * a.ldd : nullptr,
+                        Exp64(table, a.it, top[v]),
+                        Exp64(table, a.itd, a.draft ? dtop[v] : 0.0),
+                        1.0 / sum[v],
+                        off(),
+                        gone,
+                        a.draft ? 0 : turned};
+        const int x0 = k * kPart + tid * kEach;
+        double w[kEach], mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            w[i] = x0 + i < a.vocab ? left(x0 + i) : 0.0;
+            mine += w[i];
+        }
+        double up = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const double o = __shfl_up(up, d);
+            if (lane >= d)
+                up += o;
+        }
         if (tid == 0)
             found = 0x7fffffff;
-        int fallback = -1;
-        for (int i0 = 0; i0 < kPickChunk; i0 += kWalkThreads) {
-            const int x = k * kPickChunk + i0 + tid;
-            const double w = i0 + tid < kPickChunk && x < a.vocab ? left(x) : 0.0;
-            double up = w;
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_up(up, d);
-                if (lane >= d)
-                    up += o;
+        if (lane == 63)
+            wsum[wave] = up;
+        __syncthreads();
+        double at = s + (up - mine);
+        for (int i = 0; i < wave; i++)
+            at += wsum[i];
+        int hit = 0x7fffffff, some = -1;
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            at += w[i];
+            if (w[i] > 0.0) {
+                some = x0 + i;
+                if (at > aim && hit == 0x7fffffff)
+                    hit = x0 + i;
             }
-            __syncthreads();
-            if (lane == 63)
-                part[wave] = up;
-            __syncthreads();
-            double before = s;
-            for (int i = 0; i < wave; i++)
-                before += part[i];
-            if (w > 0.0 && before + up > aim)
-                atomicMin(&found, x);
-            for (int i = 0; i < kWalkThreads / 64; i++)
-                s += part[i];
-            if (w > 0.0)
-                fallback = x;
-            __syncthreads();
-            if (found != 0x7fffffff)
-                break;
         }
-        if (found == 0x7fffffff) {  // the running sum's rounding passed the aim by: the last token with a chance
+        if (hit != 0x7fffffff)
+            atomicMin(&found, hit);
+        __syncthreads();
+        token = found;
+        if (token == 0x7fffffff) {  // the running sum's rounding passed the aim by: the last token with a chance
             __syncthreads();
             if (tid == 0)
                 found = -1;
             __syncthreads();
-            atomicMax(&found, fallback);
+            atomicMax(&found, some);
             __syncthreads();
+            token = found;
         }
-        token = found;
     }
     if (tid == 0) {
         a.counts[b] = kept;
@@ -428,10 +624,10 @@ int launch_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *fi
     return check_launch("plan of drafted trees");
 }
 
-// Target and draft chunk sums, chunk maxima, and the greedy picks.
+// The walks' shares, target and draft chunk sums, chunk maxima, and the greedy picks.
 size_t tree_verify_workspace(int n, int M, int vocab) {
     const size_t cells = (size_t)2 * M * stat_chunks(vocab);
-    return up256(cells * 8) + up256(cells * 4) + up256((size_t)M * 4);
+    return up256((size_t)n * sizeof(Share)) + up256(cells * 8) + up256(cells * 4) + up256((size_t)M * 4);
 }
 
 int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
@@ -440,24 +636,46 @@ int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, 
                        int32_t *counts, int32_t *next, uint8_t *workspace) {
     const int chunks = stat_chunks(vocab);
     const size_t cells = (size_t)2 * M * chunks;
-    double *sums = (double *)workspace;
-    float *tops = (float *)(workspace + up256(cells * 8));
-    int32_t *picks = (int32_t *)(workspace + up256(cells * 8) + up256(cells * 4));
+    Share *share = (Share *)workspace;
+    double *sums = (double *)(workspace + up256((size_t)n * sizeof(Share)));
+    float *tops = (float *)((uint8_t *)sums + up256(cells * 8));
+    int32_t *picks = (int32_t *)((uint8_t *)tops + up256(cells * 4));
     const bool greedy = temperature == 0.0f;
-    WalkArgs a{logits, greedy ? nullptr : draft, uniforms, ldl,  ldd,  M,    max_nodes, vocab, chunks,
-               first,  parents, tokens, greedy ? picks : nullptr, greedy ? 0.0 : 1.0 / (double)temperature,
-               greedy || !draft ? 0.0 : 1.0 / (double)draft_temperature, tops, sums, path, counts, next};
+    const int parts = (vocab + kPart - 1) / kPart, each = kWalkGroups / n;
+    const int groups = greedy || M == 0 ? 1 : parts < each ? parts : each > 0 ? each : 1;
+    const WalkArgs a{logits,
+                     greedy ? nullptr : draft,
+                     uniforms,
+                     ldl,
+                     ldd,
+                     M,
+                     max_nodes,
+                     vocab,
+                     chunks,
+                     groups,
+                     first,
+                     parents,
+                     tokens,
+                     greedy ? picks : nullptr,
+                     greedy ? 0.0 : 1.0 / (double)temperature,
+                     greedy || !draft ? 0.0 : 1.0 / (double)draft_temperature,
+                     tops,
+                     sums,
+                     share,
+                     path,
+                     counts,
+                     next};
     if (M == 0) {  // empty trees only
     } else if (greedy) {
         if (int rc = launch_argmax(ctx, logits, ldl, M, vocab, picks, nullptr, 0, nullptr, nullptr))
             return rc;
     } else {
         verify_stats_kernel<<<dim3((unsigned)chunks, (unsigned)M, draft ? 2u : 1u), kStatThreads, 0, ctx->stream>>>(
-            logits, ldl, draft, ldd, vocab, a.it, a.itd, tops, sums);
+            logits, ldl, draft, ldd, vocab, a.it, a.itd, tops, sums, share, n);
         if (int rc = check_launch("chances of drafted tokens"))
             return rc;
     }
-    verify_walk_kernel<<<n, kWalkThreads, 0, ctx->stream>>>(a);
+    verify_walk_kernel<<<dim3((unsigned)groups, (unsigned)n), kWalkThreads, 0, ctx->stream>>>(a);
     return check_launch("verification of drafted trees");
 }
 

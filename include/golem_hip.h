@@ -670,9 +670,9 @@ int gx_qwen_attention_tree(gx_ctx *ctx, const uint16_t *qh, int n, int M, int ma
  * total (where rounding left nothing of p, p itself).  Kept tokens and the
  * next are distributed as the target's own, whatever the drafts.  An empty
  * tree gives count 0 and next -1; a row with a NaN or +inf logit, or none above
- * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule), and so
- * does a node with children whose draft row has a NaN or +inf.  Computed in
- * float64.  uniforms may be NULL at temperature 0 only.  workspace as
+ * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule); where the
+ * draft's row is such a one the walk takes no child and draws from p.  Computed
+ * in float64.  uniforms may be NULL at temperature 0 only.  workspace as
  * above; at temperature 0 the call also uses gx_argmax's scratch, with its
  * rule.  vocab at most 2^20. */
 int gx_tree_verify_workspace_bytes(int n, int M, int vocab, size_t *bytes);
