@@ -118,31 +118,37 @@ constexpr int kStatChunk = 8192;  // tokens a workgroup of the row sums takes
 constexpr int kWalkThreads = 256;
 constexpr int kPart = 2048;       // tokens a part of a running sum, eight a thread
 constexpr int kParts = kVocabMax / kPart;
+constexpr int kCells = 1280;      // chunks' statistics a walk stages at a time
 constexpr int kWalkGroups = 512;  // workgroups of a walk, over all its trees
 
-// e^((x - top) / T) as 2^(y / 32), y = (x - top) 32 / (T ln 2): n = rint(y),
-// e^((y - n) ln 2 / 32) by its Taylor series to the fifth power (the argument
-// within 0.011: 3e-15 off) times 2^(n mod 32 / 32) from a table in LDS (32
-// entries, each on banks of its own) and 2^(n div 32).  A chance below 2^-1000
-// is none, and so is that of -inf; a NaN stays one.
+// e^((x - top) / T) as 2^(y / 32), y = (x - top) 32 / (T ln 2): n = y rounded
+// by adding 1.5 * 2^52, whose low bits are then n's; 2^((y - n) / 32) by its
+// Taylor series to the fifth power (3e-15 off), times 2^(n mod 32 / 32) from a
+// table in LDS (32 entries, each on banks of its own), n div 32 added to its
+// exponent: twelve float64 operations, none of the slow kinds (rounding, ldexp
+// and int conversions).  y is held at -1023 * 32, where exponent and table
+// give the bits of zero: a chance below 2^-1022 is none, and so is that of
+// -inf.  NaN and +inf are not told apart here: their row's sum is NaN.
 struct Exp64 {
-    double A, top;
+    double A, top, least;
     const double *table;
     __device__ Exp64(const double *lds, double inv, double t)
-        : A(inv * 0x1.71547652b82fep+5), top(t == -INFINITY ? 0.0 : t), table(lds) {}
+        : A(inv * 0x1.71547652b82fep+5), top(t == -INFINITY ? 0.0 : t), table(lds) {
+        least = -32736.0 / A;
+    }
     __device__ __forceinline__ double operator()(float x) const {
-        const double y = ((double)x - top) * A;
-        const double n = __builtin_rint(y), f = y - n;
+        const double d = fmax((double)x - top, least);
+        const double z = __builtin_fma(d, A, 0x1.8p+52);
+        const double f = __builtin_fma(d, A, 0x1.8p+52 - z);
         double p = 0x1.5d87fe78a6730p-35;  // ln2^5 / 120 / 32^5, and so down
         p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-27);
         p = __builtin_fma(p, f, 0x1.c6b08d704a0bfp-20);
         p = __builtin_fma(p, f, 0x1.ebfbdff82c58ep-13);
         p = __builtin_fma(p, f, 0x1.62e42fefa39efp-6);
-        p = p * f;
-        const int ni = (int)n;
-        const double t = table[ni & 31];
-        const double e = __builtin_ldexp(__builtin_fma(t, p, t), ni >> 5);
-        return y < -32000.0 ? 0.0 : e;
+        const uint32_t n = (uint32_t)__double2loint(z);
+        const double t = table[n & 31];
+        const double s = __hiloint2double((int)((uint32_t)__double2hiint(t) + ((n & ~31u) << 15)), __double2loint(t));
+        return __builtin_fma(s * f, p, s);
     }
 };
 
@@ -164,13 +170,16 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // that finds none walking after a while ends, and so do all when the walk does.
 struct Share {
     unsigned long long claim;  // the sum's number in the high half, the next part in the low
-    unsigned fin;              // parts that are summed
-    unsigned walking, done;
-    int row, turned;
-    double top, scale, dtop, dscale;  // what is left of token x: scale e^((l_x - top) / T) - dscale e^(..)
-    double part[kParts];
+    alignas(128) unsigned fin; // parts that are summed
+    // the open sum (eight words: one load of a wavefront's lanes): the row and
+    // the tokens turned down, then the row's largest logit and the factor of its
+    // exponentials in what is left, and the draft's
+    alignas(128) unsigned long long what[8];
+    alignas(128) double part[kParts];
     int gone[kTreeNodes];
 };
+// claims before the first sum and after the last (a late asker's count stays in the low half)
+constexpr unsigned long long kWalking = 1, kWalked = 0xFFFFFFFF00000000ull;
 
 template <typename T>
 __device__ __forceinline__ T share_load(const T *p) {
@@ -198,10 +207,22 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
     exp64_table(table);
     float v[kMine];
     float top = -INFINITY;
+    if (c0 + kStatChunk <= vocab && ((uintptr_t)x & 15) == 0) {
+        typedef float v4f __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int k = 0; k < kMine; k++) {
-        const int i = c0 + tid + k * kStatThreads;
-        v[k] = i < vocab ? x[i] : -INFINITY;
+        for (int k = 0; k < kMine / 4; k++) {
+            const v4f w = __builtin_nontemporal_load((const v4f *)(x + c0) + tid + k * kStatThreads);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                v[4 * k + i] = w[i];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kMine; k++) {
+            const int i = c0 + tid + k * kStatThreads;
+            const float w = x[min(i, vocab - 1)];
+            v[k] = i < vocab ? w : -INFINITY;
+        }
     }
 #pragma unroll
     for (int k = 0; k < kMine; k++)
@@ -214,9 +235,14 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
         top = fmaxf(top, wt[w]);
     const Exp64 e(table, blockIdx.z ? itd : it, top);
     double sum = 0.0;
+    bool bad = false;
 #pragma unroll
-    for (int k = 0; k < kMine; k++)
+    for (int k = 0; k < kMine; k++) {
         sum += e(v[k]);
+        bad |= !(v[k] < INFINITY);
+    }
+    if (bad)
+        sum = NAN;
     sum = wave_sum64(sum);
     if (lane == 0)
         wsum[wave] = sum;
@@ -229,10 +255,8 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
         sums[at] = sum;
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
-        for (int b = tid; b < n; b += kStatThreads) {
+        for (int b = tid; b < n; b += kStatThreads)
             share[b].claim = 0;
-            share[b].walking = share[b].done = 0;
-        }
 }
 
 struct WalkArgs {
@@ -246,77 +270,91 @@ struct WalkArgs {
     int32_t *path, *counts, *next;
 };
 
-// The chance left to a token of a row, from both rows' logits.
+// The chance left to tokens of a row, from both rows' logits.
 struct Left {
     const float *lr, *dr;  // dr NULL: nothing of the draft's to take off
     Exp64 p, q;
     double scale, dscale;
     const int *gone;
-    int turned;
-    __device__ double operator()(int x) const {
-        double r = p(lr[x]) * scale;
+    int turned, vocab;
+    // eight tokens x0, x0 + step, ..; none past the vocabulary
+    __device__ __forceinline__ void eight(int x0, int step, double w[8]) const {
+        float l[8], d[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            l[i] = lr[min(x0 + i * step, vocab - 1)];
         if (dr) {
-            r -= q(dr[x]) * dscale;
-            return r < 0.0 ? 0.0 : r;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                d[i] = dr[min(x0 + i * step, vocab - 1)];
         }
-        for (int i = 0; i < turned; i++)
-            if (gone[i] == x)
-                r = 0.0;
-        return r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            double r = p(l[i]) * scale;
+            if (dr)
+                r -= q(d[i]) * dscale;
+            w[i] = r < 0.0 || x0 + i * step >= vocab ? 0.0 : r;
+        }
+        for (int k = 0; k < turned; k++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                w[i] = gone[k] == x0 + i * step ? 0.0 : w[i];
     }
 };
 
 // One part's sum, by the whole workgroup (every thread gets it): eight tokens
 // a thread, a wavefront's 64 tokens in a row.
-__device__ __forceinline__ double part_sum(const Left &left, int k, int vocab, double *wsum) {
-    const int tid = threadIdx.x, x0 = k * kPart + tid;
-    double s = 0.0;
-#pragma unroll
-    for (int i = 0; i < kPart / kWalkThreads; i++)
-        if (x0 + i * kWalkThreads < vocab)
-            s += left(x0 + i * kWalkThreads);
+__device__ __forceinline__ double part_sum(const Left &left, int k, double *wsum) {
+    const int tid = threadIdx.x;
+    double w[8];
+    left.eight(k * kPart + tid, kWalkThreads, w);
+    double s = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     s = wave_sum64(s);
     __syncthreads();
     if ((tid & 63) == 0)
         wsum[tid >> 6] = s;
     __syncthreads();
     s = wsum[0];
-    for (int w = 1; w < kWalkThreads / 64; w++)
-        s += wsum[w];
+    for (int i = 1; i < kWalkThreads / 64; i++)
+        s += wsum[i];
     return s;
 }
 
-// One part of the sum that is open, workgroup-wide; false where the claim came
-// after the last.
+// The part of the open sum that `old`, a claim of this workgroup, names; false
+// where the claim came after the last.
 struct Helper {
     const WalkArgs &a;
     Share &sh;
     const double *table;
     double *wsum;
+    unsigned long long *what;
     int *gone;
     int parts;
-    __device__ bool one(unsigned long long old) {  // old: a claim of this workgroup, the same in every thread
-        const int k = (int)(unsigned)old;
+    __device__ __forceinline__ bool one(unsigned long long old) {
+        const int tid = threadIdx.x, k = (int)(unsigned)old;
         if (k >= parts)
             return false;
-        const int row = share_load(&sh.row), turned = share_load(&sh.turned);
-        const double dscale = share_load(&sh.dscale);
-        const Left left{a.logits + (size_t)row * a.ldl,
-                        dscale > 0.0 ? a.draft + (size_t)row * a.ldd : nullptr,
-                        Exp64(table, a.it, share_load(&sh.top)),
-                        Exp64(table, a.itd, share_load(&sh.dtop)),
-                        share_load(&sh.scale),
-                        dscale,
-                        gone,
-                        a.draft ? 0 : turned};
-        if (!a.draft) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < turned; i += kWalkThreads)
+        if (tid < 8)
+            what[tid] = share_load(&sh.what[tid]);
+        __syncthreads();
+        const int row = (int)what[0], turned = (int)what[1];
+        const double dscale = __longlong_as_double((long long)what[5]);
+        if (turned > 0) {
+            for (int i = tid; i < turned; i += kWalkThreads)
                 gone[i] = share_load(&sh.gone[i]);
             __syncthreads();
         }
-        const double s = part_sum(left, k, a.vocab, wsum);
-        if (threadIdx.x == 0) {
+        const Left left{a.logits + (size_t)row * a.ldl,
+                        dscale > 0.0 ? a.draft + (size_t)row * a.ldd : nullptr,
+                        Exp64(table, a.it, __longlong_as_double((long long)what[2])),
+                        Exp64(table, a.itd, __longlong_as_double((long long)what[4])),
+                        __longlong_as_double((long long)what[3]),
+                        dscale,
+                        gone,
+                        turned,
+                        a.vocab};
+        const double s = part_sum(left, k, wsum);
+        if (tid == 0) {
             share_store(&sh.part[k], s);
             __hip_atomic_fetch_add(&sh.fin, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -332,40 +370,43 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     __shared__ double px[kTreeNodes], qx[kTreeNodes];                        // a node's token by its parent's rows
     __shared__ double top[kTreeNodes], sum[kTreeNodes], dtop[kTreeNodes], dsum[kTreeNodes];  // a node's own rows
     __shared__ double run[kParts], table[32], wsum[kWalkThreads / 64];
-    __shared__ unsigned long long got;
+    __shared__ double csum[kCells];
+    __shared__ float ctop[kCells];
+    __shared__ unsigned long long got, what[8];
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y;
     const int f0 = min(max(a.first[b], 0), a.M), T = min(min(max(a.first[b + 1], f0), a.M) - f0, a.max_nodes);
     const int parts = (a.vocab + kPart - 1) / kPart;
     Share &sh = a.share[b];
-    Helper help{a, sh, table, wsum, gone, parts};
+    Helper help{a, sh, table, wsum, what, gone, parts};
     if (blockIdx.x > 0) {
         if (T <= 0)
             return;
         exp64_table(table);
-        unsigned spent = 0;
+        int spent = 0;
         for (;;) {
             __syncthreads();
             if (tid == 0) {
-                unsigned long long c = ~0ull;  // nothing more comes
+                unsigned long long c;
                 for (;;) {
-                    if (share_load(&sh.done))
-                        break;
-                    if (!share_load(&sh.walking) && ++spent > kPolls)
-                        break;
                     c = share_load(&sh.claim);
+                    if (c >> 32 == kWalked >> 32)
+                        break;
+                    if (c == 0 && ++spent > kPolls) {
+                        c = kWalked;
+                        break;
+                    }
                     if (c >> 32 && (unsigned)c < (unsigned)parts) {
                         c = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
                         break;
                     }
-                    c = ~0ull;
-                    __builtin_amdgcn_s_sleep(4);
+                    __builtin_amdgcn_s_sleep(8);
                 }
                 got = c;
             }
             __syncthreads();
             const unsigned long long mine = got;
-            if (mine == ~0ull)
+            if (mine >> 32 == kWalked >> 32)
                 return;
             help.one(mine);
         }
@@ -381,7 +422,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         return;
     }
     if (tid == 0 && !a.picks)
-        share_store(&sh.walking, 1u);
+        share_store(&sh.claim, kWalking);
     exp64_table(table);
     for (int i = tid; i < T; i += kWalkThreads) {
         par[i] = a.parents[f0 + i];
@@ -405,24 +446,35 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         return;
     }
-    // every row's statistics from its chunks', then every child's chances
-    for (int i = tid; i < T * 2; i += kWalkThreads) {
-        const int node = i >> 1, z = i & 1;
-        if (z && !a.draft)
-            continue;
-        const size_t at = ((size_t)z * a.M + f0 + node) * a.chunks;
-        float mx = -INFINITY;
-        for (int c = 0; c < a.chunks; c++)
-            mx = fmaxf(mx, a.tops[at + c]);
-        const Exp64 e(table, z ? a.itd : a.it, mx);
-        double s = 0.0;
-        for (int c = 0; c < a.chunks; c++)
-            if (a.sums[at + c] != 0.0)
-                s += a.tops[at + c] == -INFINITY ? a.sums[at + c] : a.sums[at + c] * e(a.tops[at + c]);
-        (z ? dtop : top)[node] = mx;
-        (z ? dsum : sum)[node] = s;
+    // every row's statistics from its chunks' (staged in LDS, so many rows' at a
+    // time), then every child's chances
+    const int rows = a.draft ? 2 * T : T, batch = max(1, kCells / a.chunks);
+    for (int r0 = 0; r0 < rows; r0 += batch) {
+        const int here = min(batch, rows - r0);
+        for (int i = tid; i < here * a.chunks; i += kWalkThreads) {
+            const int row = r0 + i / a.chunks, z = row >= T;
+            const size_t at = ((size_t)z * a.M + f0 + (z ? row - T : row)) * a.chunks + i % a.chunks;
+            ctop[i] = a.tops[at];
+            csum[i] = a.sums[at];
+        }
+        __syncthreads();
+        for (int i = tid; i < here; i += kWalkThreads) {
+            const int row = r0 + i, z = row >= T, node = z ? row - T : row;
+            float mx = -INFINITY;
+            for (int c = 0; c < a.chunks; c++)
+                mx = fmaxf(mx, ctop[i * a.chunks + c]);
+            const Exp64 e(table, z ? a.itd : a.it, mx);
+            double s = 0.0;
+            for (int c = 0; c < a.chunks; c++) {
+                const double cs = csum[i * a.chunks + c];
+                if (cs != 0.0)
+                    s += cs - cs == 0.0 ? cs * e(ctop[i * a.chunks + c]) : cs;
+            }
+            (z ? dtop : top)[node] = mx;
+            (z ? dsum : sum)[node] = s;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     for (int m = tid; m < T; m += kWalkThreads) {
         const int p = par[m], x = tok[m];
         if (p < 0 || p >= m || x < 0 || x >= a.vocab)
@@ -432,113 +484,120 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             qx[m] = Exp64(table, a.itd, dtop[p])(a.draft[(size_t)(f0 + p) * a.ldd + x]) / dsum[p];
     }
     __syncthreads();
-    double c = 0.0, tried = 0.0, mass = 1.0;
-    int turned = 0;
+    double c = 0.0, tried = 0.0, mass = 1.0, all = 0.0;
+    int turned = 0, m = 1;
     unsigned sums = 0;
-    bool known = true;   // mass is up to date
-    bool summed = false; // run[] holds the parts of what is left
+    bool known = true;    // mass is up to date
+    bool summed = false;  // run[] holds the parts of what is left
     // the factor of the draft's exponentials in what is left (a row of q that is
     // none takes nothing off)
-    auto off = [&]() {
+    auto off = [&]() __attribute__((always_inline)) {
         const double d = a.draft ? c / dsum[v] : 0.0;
         return d > 0.0 && d - d == 0.0 ? d : 0.0;
     };
-    // the sum of what is left of v's row
-    auto total = [&]() {
-        if (tid == 0) {
-            share_store(&sh.row, f0 + v);
-            share_store(&sh.turned, turned);
-            share_store(&sh.top, top[v]);
-            share_store(&sh.scale, 1.0 / sum[v]);
-            share_store(&sh.dtop, a.draft ? dtop[v] : 0.0);
-            share_store(&sh.dscale, off());
-            for (int i = 0; i < turned; i++)
-                share_store(&sh.gone[i], gone[i]);
-            share_store(&sh.fin, 0u);
-            __hip_atomic_store(&sh.claim, (unsigned long long)++sums << 32, __ATOMIC_RELEASE,
-                               __HIP_MEMORY_SCOPE_AGENT);
-        }
-        for (;;) {
-            __syncthreads();
-            if (tid == 0)
-                got = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
-            __syncthreads();
-            if (!help.one(got))
-                break;
-        }
-        if (tid == 0)
-            while (__hip_atomic_load(&sh.fin, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) < (unsigned)parts)
-                __builtin_amdgcn_s_sleep(1);
-        __syncthreads();
-        for (int k = tid; k < parts; k += kWalkThreads)
-            run[k] = share_load(&sh.part[k]);
-        __syncthreads();
-        double s = 0.0;
-        for (int k = 0; k < parts; k++)
-            s += run[k];
-        summed = true;
-        return s;
-    };
-    for (int m = 1; m < T; m++) {
-        if (par[m] != v)
-            continue;
-        const int x = tok[m];
-        bool over = x < 0 || x >= a.vocab;  // no token, or one turned down already: passed over
-        for (int i = 0; i < turned; i++)
-            over |= gone[i] == x;
-        if (over)
-            continue;
-        const double u = (double)a.uniforms[f0 + m];
-        bool take;
-        if (a.draft) {
-            const double rest = 1.0 - tried;
-            if (!known)
-                mass = total();
-            known = true;
-            if (!(rest > 0.0) || !(mass > 0.0))
-                continue;  // nothing a draft could have come from is left
-            const double r = px[m] - c * qx[m];
-            take = u * mass * qx[m] < (r < 0.0 ? 0.0 : r) * rest;
-            if (!take) {
-                c += mass / rest;
-                tried += qx[m];
-                known = summed = false;
+    for (;;) {
+        // down the tree, until a sum is wanted or the nodes are at their end
+        while (m < T) {
+            const int x = tok[m];
+            bool over = par[m] != v || x < 0 || x >= a.vocab;  // no child, or no token
+            for (int i = 0; !over && i < turned; i++)
+                over = gone[i] == x;  // one turned down already
+            if (over) {
+                m++;
+                continue;
             }
-        } else {
-            take = u * mass < px[m];
-            if (!take)
-                mass -= px[m];
+            const double u = (double)a.uniforms[f0 + m];
+            bool take;
+            if (a.draft) {
+                if (!known)
+                    break;
+                const double rest = 1.0 - tried;
+                if (!(rest > 0.0) || !(mass > 0.0)) {  // nothing a draft could have come from is left
+                    m++;
+                    continue;
+                }
+                const double r = px[m] - c * qx[m];
+                take = u * mass * qx[m] < (r < 0.0 ? 0.0 : r) * rest;
+                if (!take) {
+                    c += mass / rest;
+                    tried += qx[m];
+                    known = summed = false;
+                }
+            } else {
+                take = u * mass < px[m];
+                if (!take)
+                    mass -= px[m];
+            }
+            __syncthreads();
+            if (take) {
+                if (tid == 0)
+                    path[kept] = m;
+                v = m;
+                kept++;
+                c = tried = 0.0;
+                mass = 1.0;
+                turned = 0;
+                known = true;
+                summed = false;
+            } else {
+                if (tid == 0)
+                    gone[turned] = x;
+                turned++;
+            }
+            __syncthreads();
+            m++;
         }
-        __syncthreads();
-        if (take) {
+        const bool ending = m >= T;
+        if (!summed) {
+            // the sum of what is left of v's row, handed out
+            if (tid == 0) {
+                const int listed = a.draft ? 0 : turned;
+                const double words[] = {1.0 / sum[v], off()};
+                share_store(&sh.what[0], (unsigned long long)(f0 + v));
+                share_store(&sh.what[1], (unsigned long long)listed);
+                share_store(&sh.what[2], (unsigned long long)__double_as_longlong(top[v]));
+                share_store(&sh.what[3], (unsigned long long)__double_as_longlong(words[0]));
+                share_store(&sh.what[4], (unsigned long long)__double_as_longlong(a.draft ? dtop[v] : 0.0));
+                share_store(&sh.what[5], (unsigned long long)__double_as_longlong(words[1]));
+                for (int i = 0; i < listed; i++)
+                    share_store(&sh.gone[i], gone[i]);
+                share_store(&sh.fin, 0u);
+                __hip_atomic_store(&sh.claim, (unsigned long long)++sums << 32, __ATOMIC_RELEASE,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+            }
+            for (;;) {
+                __syncthreads();
+                if (tid == 0)
+                    got = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                if (!help.one(got))
+                    break;
+            }
             if (tid == 0)
-                path[kept] = m;
-            v = m;
-            kept++;
-            c = tried = 0.0;
-            mass = 1.0;
+                while (__hip_atomic_load(&sh.fin, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) < (unsigned)parts)
+                    __builtin_amdgcn_s_sleep(1);
+            __syncthreads();
+            for (int k = tid; k < parts; k += kWalkThreads)
+                run[k] = share_load(&sh.part[k]);
+            __syncthreads();
+            summed = known = true;
+        }
+        all = 0.0;
+        for (int k = 0; k < parts; k++)
+            all += run[k];
+        mass = all;
+        if (!ending)
+            continue;
+        if (all == 0.0 && (c > 0.0 || turned > 0)) {  // rounding left nothing: the row as it was
+            c = 0.0;
             turned = 0;
-            known = true;
             summed = false;
-        } else {
-            if (tid == 0)
-                gone[turned] = x;
-            turned++;
+            continue;
         }
-        __syncthreads();
-    }
-    double all = 0.0;
-    for (int k = 0; summed && k < parts; k++)
-        all += run[k];
-    if (!summed)
-        all = total();
-    if (all == 0.0 && (c > 0.0 || turned > 0)) {  // rounding left nothing: the row as it was
-        c = 0.0;
-        turned = 0;
-        all = total();
+        break;
     }
     if (tid == 0)
-        share_store(&sh.done, 1u);
+        share_store(&sh.claim, kWalked);
     int token = -1;
     if (all > 0.0 && all - all == 0.0) {
         const double aim = (double)a.uniforms[f0] * all;
@@ -551,6 +610,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             s += run[k];
         // the part's running sum: eight tokens in a row a thread
         constexpr int kEach = kPart / kWalkThreads;
+        static_assert(kEach == 8, "Left::eight");
         const Left left{a.logits + (size_t)(f0 + v) * a.ldl,
                         off() > 0.0 ? a.draft + (size_t)(f0 + v) * a.ldd : nullptr,
                         Exp64(table, a.it, top[v]),
@@ -558,14 +618,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                         1.0 / sum[v],
                         off(),
                         gone,
-                        a.draft ? 0 : turned};
+                        a.draft ? 0 : turned,
+                        a.vocab};
         const int x0 = k * kPart + tid * kEach;
         double w[kEach], mine = 0.0;
+        left.eight(x0, 1, w);
 #pragma unroll
-        for (int i = 0; i < kEach; i++) {
-            w[i] = x0 + i < a.vocab ? left(x0 + i) : 0.0;
+        for (int i = 0; i < kEach; i++)
             mine += w[i];
-        }
         double up = mine;
         for (int d = 1; d < 64; d <<= 1) {
             const double o = __shfl_up(up, d);

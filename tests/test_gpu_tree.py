@@ -503,7 +503,7 @@ def test_verify(dev, sizes, fanout, V, pad, form):
 def test_verify_temperatures_apart(dev):
     """A draft temperature of its own, and temperatures that leave one token or all alike."""
     sizes = [20, 9]
-    for t, td in ((0.05, 0.5), (1.7, 0.6), (40.0, 3.0)):
+    for t, td in ((0.05, 0.5), (1.7, 0.6), (40.0, 3.0), (1e-12, 1e-10), (1e30, 1e20)):
         parents, tokens, logits, draft, u = make_verify(40, sizes, 4, 300, True)
         args = (sizes, parents, tokens, logits, draft, t, td, u, 20)
         for x, y in zip(run_verify(dev, *args), verify_reference(*args)):
