@@ -369,9 +369,10 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     __shared__ int par[kTreeNodes], tok[kTreeNodes], gone[kTreeNodes];
     __shared__ double px[kTreeNodes], qx[kTreeNodes];                        // a node's token by its parent's rows
     __shared__ double top[kTreeNodes], sum[kTreeNodes], dtop[kTreeNodes], dsum[kTreeNodes];  // a node's own rows
-    __shared__ double run[kParts], table[32], wsum[kWalkThreads / 64];
+    __shared__ double run[kParts], own[kParts], table[32], wsum[kWalkThreads / 64];
     __shared__ double csum[kCells];
     __shared__ float ctop[kCells];
+    __shared__ float un[kTreeNodes];
     __shared__ unsigned long long got, what[8];
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y;
@@ -427,6 +428,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     for (int i = tid; i < T; i += kWalkThreads) {
         par[i] = a.parents[f0 + i];
         tok[i] = a.tokens[f0 + i];
+        if (!a.picks)
+            un[i] = a.uniforms[f0 + i];
     }
     __syncthreads();  // (and the path's -1s are written)
     if (tid == 0)
@@ -461,6 +464,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         for (int i = tid; i < here; i += kWalkThreads) {
             const int row = r0 + i, z = row >= T, node = z ? row - T : row;
             float mx = -INFINITY;
+#pragma unroll 4
             for (int c = 0; c < a.chunks; c++)
                 mx = fmaxf(mx, ctop[i * a.chunks + c]);
             const Exp64 e(table, z ? a.itd : a.it, mx);
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 m++;
                 continue;
             }
-            const double u = (double)a.uniforms[f0 + m];
+            const double u = (double)un[m];
             bool take;
             if (a.draft) {
                 if (!known)
@@ -577,14 +581,30 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 while (__hip_atomic_load(&sh.fin, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) < (unsigned)parts)
                     __builtin_amdgcn_s_sleep(1);
             __syncthreads();
-            for (int k = tid; k < parts; k += kWalkThreads)
-                run[k] = share_load(&sh.part[k]);
+            // the parts' running sum: two of them a thread, over the wavefronts
+            static_assert(kParts == 2 * kWalkThreads, "two parts a thread");
+            const double one = 2 * tid < parts ? share_load(&sh.part[2 * tid]) : 0.0;
+            const double two = 2 * tid + 1 < parts ? share_load(&sh.part[2 * tid + 1]) : 0.0;
+            double up = one + two;
+            for (int d = 1; d < 64; d <<= 1) {
+                const double o = __shfl_up(up, d);
+                if (lane >= d)
+                    up += o;
+            }
+            if (lane == 63)
+                wsum[wave] = up;
+            __syncthreads();
+            double at = 0.0;
+            for (int i = 0; i < wave; i++)
+                at += wsum[i];
+            run[2 * tid] = at + (up - two);
+            run[2 * tid + 1] = at + up;
+            own[2 * tid] = one;
+            own[2 * tid + 1] = two;
             __syncthreads();
             summed = known = true;
         }
-        all = 0.0;
-        for (int k = 0; k < parts; k++)
-            all += run[k];
+        all = run[parts - 1];
         mass = all;
         if (!ending)
             continue;
@@ -600,14 +620,30 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         share_store(&sh.claim, kWalked);
     int token = -1;
     if (all > 0.0 && all - all == 0.0) {
-        const double aim = (double)a.uniforms[f0] * all;
-        double s = 0.0;
-        int k = 0, last = 0;
-        for (int i = 0; i < parts; i++)
-            if (run[i] > 0.0)
-                last = i;
-        for (; k < last && s + run[k] <= aim; k++)
-            s += run[k];
+        const double aim = (double)un[0] * all;
+        // the first part that adds to the running sum and at whose end it is past
+        // the aim, or the last that adds to it
+        if (tid == 0)
+            found = 0x7fffffff;
+        __syncthreads();
+        int k = -1;
+        for (int i = tid; i < parts; i += kWalkThreads)
+            if (own[i] > 0.0) {
+                k = i;
+                if (run[i] > aim)
+                    atomicMin(&found, i);
+            }
+        __syncthreads();
+        if (found == 0x7fffffff) {
+            __syncthreads();
+            if (tid == 0)
+                found = -1;
+            __syncthreads();
+            atomicMax(&found, k);
+            __syncthreads();
+        }
+        k = found;
+        const double s = k > 0 ? run[k - 1] : 0.0;
         // the part's running sum: eight tokens in a row a thread
         constexpr int kEach = kPart / kWalkThreads;
         static_assert(kEach == 8, "Left::eight");
@@ -632,6 +668,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             if (lane >= d)
                 up += o;
         }
+        __syncthreads();
         if (tid == 0)
             found = 0x7fffffff;
         if (lane == 63)
