@@ -118,7 +118,7 @@ constexpr int kStatChunk = 8192;  // tokens a workgroup of the row sums takes
 constexpr int kWalkThreads = 256;
 constexpr int kPart = 2048;       // tokens a part of a running sum, eight a thread
 constexpr int kParts = kVocabMax / kPart;
-constexpr int kCells = 1280;      // chunks' statistics a walk stages at a time
+constexpr int kCells = 1536;      // chunks' statistics a walk stages at a time
 constexpr int kWalkGroups = 512;  // workgroups of a walk, over all its trees
 
 // e^((x - top) / T) as 2^(y / 32), y = (x - top) 32 / (T ln 2): n = y rounded
@@ -189,6 +189,16 @@ template <typename T>
 __device__ __forceinline__ void share_store(T *p, T v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+
+template <typename T>
+__device__ __forceinline__ T share_add(T *p, T v) {
+    return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Everything before it done, for every XCD, before anything after: all that the
+// workgroups share goes through the two calls above, past the caches that are
+// not coherent, so waiting for them is enough.  (Agent-scope release and acquire
+// would write back and drop the XCD's L2 each time: 20 us a sum in place of 5.)
+__device__ __forceinline__ void share_order() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // grid (chunks, M, 1 or 2): a chunk's largest logit and sum of exponentials,
 // of the target's rows (z 0) and the draft's; and the walks' shares cleared.
@@ -356,7 +366,8 @@ struct Helper {
         const double s = part_sum(left, k, wsum);
         if (tid == 0) {
             share_store(&sh.part[k], s);
-            __hip_atomic_fetch_add(&sh.fin, 1u, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_AGENT);
+            share_order();
+            share_add(&sh.fin, 1u);
         }
         return true;
     }
@@ -398,12 +409,13 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                         break;
                     }
                     if (c >> 32 && (unsigned)c < (unsigned)parts) {
-                        c = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
+                        c = share_add(&sh.claim, 1ull);
                         break;
                     }
                     __builtin_amdgcn_s_sleep(8);
                 }
                 got = c;
+                share_order();
             }
             __syncthreads();
             const unsigned long long mine = got;
@@ -454,11 +466,21 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     const int rows = a.draft ? 2 * T : T, batch = max(1, kCells / a.chunks);
     for (int r0 = 0; r0 < rows; r0 += batch) {
         const int here = min(batch, rows - r0);
-        for (int i = tid; i < here * a.chunks; i += kWalkThreads) {
-            const int row = r0 + i / a.chunks, z = row >= T;
-            const size_t at = ((size_t)z * a.M + f0 + (z ? row - T : row)) * a.chunks + i % a.chunks;
-            ctop[i] = a.tops[at];
-            csum[i] = a.sums[at];
+        // (the target's rows of a tree follow one another, and so do the draft's)
+        const int c0 = r0 * a.chunks, split = T * a.chunks, last = (r0 + here) * a.chunks - 1;
+        float ct[kCells / kWalkThreads];
+        double cs[kCells / kWalkThreads];
+#pragma unroll
+        for (int k = 0; k < kCells / kWalkThreads; k++) {
+            const int i = min(c0 + tid + k * kWalkThreads, last);
+            const size_t at = i < split ? (size_t)f0 * a.chunks + i : (size_t)(a.M + f0) * a.chunks + (i - split);
+            ct[k] = a.tops[at];
+            cs[k] = a.sums[at];
+        }
+#pragma unroll
+        for (int k = 0; k < kCells / kWalkThreads; k++) {
+            ctop[tid + k * kWalkThreads] = ct[k];
+            csum[tid + k * kWalkThreads] = cs[k];
         }
         __syncthreads();
         for (int i = tid; i < here; i += kWalkThreads) {
@@ -566,20 +588,21 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 for (int i = 0; i < listed; i++)
                     share_store(&sh.gone[i], gone[i]);
                 share_store(&sh.fin, 0u);
-                __hip_atomic_store(&sh.claim, (unsigned long long)++sums << 32, __ATOMIC_RELEASE,
-                                   __HIP_MEMORY_SCOPE_AGENT);
+                share_order();
+                share_store(&sh.claim, (unsigned long long)++sums << 32);
             }
             for (;;) {
                 __syncthreads();
                 if (tid == 0)
-                    got = __hip_atomic_fetch_add(&sh.claim, 1ull, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT);
+                    got = share_add(&sh.claim, 1ull);
                 __syncthreads();
                 if (!help.one(got))
                     break;
             }
             if (tid == 0)
-                while (__hip_atomic_load(&sh.fin, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_AGENT) < (unsigned)parts)
+                while (share_load(&sh.fin) < (unsigned)parts)
                     __builtin_amdgcn_s_sleep(1);
+            share_order();
             __syncthreads();
             // the parts' running sum: two of them a thread, over the wavefronts
             static_assert(kParts == 2 * kWalkThreads, "two parts a thread");
