@@ -29,12 +29,17 @@ namespace {
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
-constexpr int kWaves = 4;        // wavefronts a workgroup, each with a share of its tiles
-constexpr int kTile = 32;        // keys a step
+constexpr int kTile = 32;        // rows a wavefront
+constexpr int kStage = 64;       // keys a step
+constexpr int kMaxWaves = 8;     // wavefronts a workgroup: a tile of rows each, the keys shared
 constexpr int kMaxSplits = 64;   // shares of the keys, over workgroups
-constexpr float kShift = 10.0f;  // probabilities are held times 2^10, their low parts clear of fp16's subnormals
+// Probabilities are held times 2^8, their low parts clear of fp16's
+// subnormals, and the reference the exponent is taken from follows the maximum
+// only when that has risen by 2^7: still below fp16's largest.
+constexpr float kShift = 8.0f, kRise = 7.0f;
 
 struct Args {
     const uint16_t *qh;
@@ -51,14 +56,14 @@ struct Args {
 
 // A tree's tokens, cached positions and steps, the same for every kernel.
 struct Tree {
-    int f0, T, P, a, np, total, per;
+    int f0, T, P, a, np, total, per;  // (total and per: steps)
     __device__ Tree(const Args &x, int b) {
         f0 = min(max(x.first[b], 0), x.M);
         T = min(min(max(x.first[b + 1], f0), x.M) - f0, x.max_nodes);
         P = min(max(x.prefix[b], 0), min(x.max_prefix, x.context));
         a = f0 & 7;  // draft rows are read from a multiple of 8
-        np = (P + kTile - 1) / kTile;
-        total = np + (T > 0 ? (a + T + kTile - 1) / kTile : 0);
+        np = (P + kStage - 1) / kStage;
+        total = np + (T > 0 ? (a + T + kStage - 1) / kStage : 0);
         per = max(1, (total + x.S - 1) / x.S);
     }
 };
@@ -74,25 +79,64 @@ __device__ __forceinline__ v8h keep(v8h v, int lo, int hi) {
     return r;
 }
 
-// grid (kv_heads, 32-row tiles, trees * S): key-value heads fastest, so that
-// with eight of them every workgroup of a head is on one XCD and shares its L2.
+__device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
+// grid (kv_heads, row groups, trees * S), 64 threads a 32-row tile of the
+// group: key-value heads fastest, so that with eight of them every workgroup
+// of a head is on one XCD and shares its L2.
+//
+// A step's 64 keys and values come into LDS by direct loads, one step ahead of
+// the products, for every tile of the group: the keys as 1 KiB pieces of 64
+// positions, a value row's 128 bytes with its eight 16-byte chunks exchanged
+// by the row's low bits, so that both the loads (eight whole rows each) and
+// the operand reads (a chunk of 32 rows) are without conflicts.
 template <int HD>
-__global__ __launch_bounds__(64 * kWaves) void attn_tree_kernel(const Args x) {
-    constexpr int KS = HD / 16, ET = HD / 32;
-    __shared__ float ms[kWaves][kTile], ls[kWaves][kTile];
-    __shared__ float os[kTile][HD + 1];
+__global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x) {
+    constexpr int KS = HD / 16, ET = HD / 32, kSlot = HD * 256;
+    extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int li = lane & 31, h = lane >> 5;
+    const int nw = blockDim.x >> 6, li = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
     const Tree t(x, b);
-    const int g = x.heads / x.kv_heads, R = t.T * g, r0 = blockIdx.y * kTile;
+    const int g = x.heads / x.kv_heads, R = t.T * g, g0 = blockIdx.y * nw * kTile, r0 = g0 + wave * kTile;
     const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
-    if (r0 >= R || t0 >= t1)
+    if (g0 >= R || t0 >= t1)
         return;
     const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
     const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
     const uint16_t *kc = x.kc + cache, *vc = x.vc + cache;
     const uint16_t *kd = x.kd + (size_t)kvh * HD * x.draft_context, *vd = x.vd + (size_t)kvh * HD * x.draft_context;
+
+    // step j's rows: where they begin, and which of them there are
+    auto rows_of = [&](int j, int &p0, int &lo, int &hi) __attribute__((always_inline)) {
+        const bool draft = j >= t.np;
+        p0 = draft ? t.f0 - t.a + kStage * (j - t.np) : kStage * j;
+        lo = draft ? t.f0 : 0;
+        hi = draft ? t.f0 + t.T : t.P;
+        return draft;
+    };
+    auto load = [&](int j, uint8_t *to) __attribute__((always_inline)) {
+        int p0, lo, hi;
+        const bool draft = rows_of(j, p0, lo, hi);
+        const int rows = draft ? x.draft_context : x.context;
+        const char *kb = (const char *)(draft ? kd : kc), *vb = (const char *)(draft ? vd : vc);
+        const uint32_t kp = (uint32_t)min(max(p0 + lane, lo), hi - 1) * 16;
+        const uint32_t vp = ((uint32_t)(lane >> 3) * rows + min(p0 + 8 * ((lane & 7) ^ (lane >> 3)), rows - 8)) * 2;
+        // (a uniform base and the lane's 32-bit offset: no vector instruction a load)
+        for (int i = wave; i < HD / 8; i += nw) {
+            const char *src = kb + (size_t)i * rows * 16;
+            asm("" : "+s"(src));
+            __builtin_amdgcn_global_load_lds(src + kp, (lds_ptr)(to + i * 1024), 16, 0, 0);
+        }
+        for (int i = wave; i < HD / 8; i += nw) {
+            const char *src = vb + (size_t)i * rows * 16;
+            asm("" : "+s"(src));
+            __builtin_amdgcn_global_load_lds(src + vp, (lds_ptr)(to + HD * 128 + i * 1024), 16, 0, 0);
+        }
+    };
+    load(t0, lds);
 
     const int r = min(r0 + li, R - 1), node = r / g;
     const uint16_t *qr = x.qh + ((size_t)(t.f0 + node) * x.heads + kvh * g + (r - node * g)) * HD + 8 * h;
@@ -101,122 +145,123 @@ __global__ __launch_bounds__(64 * kWaves) void attn_tree_kernel(const Args x) {
     for (int s = 0; s < KS; s++)
         q[s] = *(const v8h *)(qr + 16 * s);
     const uint32_t *mrow = x.mask + (size_t)(t.f0 + node) * x.words;
-    const int lis = (li & ~12) | ((li & 4) << 1) | ((li & 8) >> 1);
+    const uint32_t klane = h * 1024 + ((li & ~12) | ((li & 4) << 1) | ((li & 8) >> 1)) * 16;
+    const uint32_t vlane = HD * 128 + li * 128, vx = h ^ (li & 7);
 
     v16f o[ET] = {};
-    float m = -INFINITY, l = 0.0f;
-    for (int j = t0 + wave; j < t1; j += kWaves) {
-        const bool draft = j >= t.np;
-        const int d = j - t.np;
-        // the tile's first row and its rows' range, in the cache or the draft buffers
-        const int p0 = draft ? t.f0 - t.a + kTile * d : kTile * j;
-        const int lo = draft ? t.f0 : 0, hi = draft ? t.f0 + t.T : t.P;
-        const uint16_t *kb = draft ? kd : kc, *vb = draft ? vd : vc;
-        const int rows = draft ? x.draft_context : x.context;
-        const int kp = min(max(p0 + lis, lo), hi - 1);
-        v16f s = {};
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const v8h a = *(const v8h *)(kb + ((size_t)(2 * k + h) * rows + kp) * 8);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], s, 0, 0, 0);
+    float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
+    int at = 0;
+    for (int j = t0; j < t1; j++, at = kSlot - at) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        lds_barrier();
+        if (j + 1 < t1)
+            load(j + 1, lds + (kSlot - at));
+        uint8_t *st = lds + at;
+        int p0, lo, hi;
+        const bool draft = rows_of(j, p0, lo, hi);
+        if (p0 < lo || p0 + kStage > hi) {  // rows of the step that there are not: their values become zero
+            for (int i = tid; i < HD * 8; i += 64 * nw) {
+                const int e = i >> 3, pv = p0 + 8 * ((i & 7) ^ (e & 7));
+                if (pv < lo || pv + 8 > hi) {
+                    v8h *to = (v8h *)(st + HD * 128 + i * 16);
+                    *to = keep(*to, lo - pv, hi - pv);
+                }
+            }
+            lds_barrier();
         }
-        v8h v[ET][2];
+        if (r0 >= R)
+            continue;
+        v16f s[2] = {};
 #pragma unroll
-        for (int et = 0; et < ET; et++)
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v8h a = *(const v8h *)(st + klane + 2048 * k + 512 * u);
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], s[u], 0, 0, 0);
+            }
+        if (draft || p0 + kStage > hi) {
+            uint32_t sees[2] = {~0u, ~0u};
+            if (draft) {
+                const int w0 = 2 * (j - t.np);  // bits from node 32 w0 - a on
+                uint32_t w[3];
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+                    w[i] = w0 + i > 0 && w0 + i <= x.words ? mrow[w0 + i - 1] : 0u;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+                    sees[u] = t.a ? (w[u + 1] << t.a) | (w[u] >> (32 - t.a)) : w[u + 1];
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++)
-                v[et][u] = *(const v8h *)(vb + (size_t)(32 * et + li) * rows + min(p0 + 16 * u + 8 * h, rows - 8));
-        uint32_t sees = ~0u;
-        if (draft) {
-            const uint32_t w = d < x.words ? mrow[d] : 0u;
-            sees = t.a ? (w << t.a) | (d > 0 ? mrow[d - 1] >> (32 - t.a) : 0u) : w;
-        }
-        if (p0 < lo || p0 + kTile > hi) {  // the tile's rows outside the range: not seen, their values zero
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int pv = p0 + 16 * u + 8 * h;
-#pragma unroll
-                for (int et = 0; et < ET; et++)
-                    v[et][u] = keep(v[et][u], lo - pv, hi - pv);
-            }
-            const int below = max(lo - p0, 0), above = min(hi - p0, kTile);
-            sees &= (above >= 32 ? ~0u : (1u << above) - 1) & ~((1u << below) - 1);
+                for (int i = 0; i < 16; i++) {
+                    const int k = 16 * (i >> 3) + 8 * h + (i & 7), p = p0 + 32 * u + k;
+                    s[u][i] = (sees[u] >> k & 1) && p >= lo && p < hi ? s[u][i] : -INFINITY;
+                }
         }
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int k = 16 * (i >> 3) + 8 * h + (i & 7);
-            s[i] = sees >> k & 1 ? s[i] * x.c : -INFINITY;
-            mx = fmaxf(mx, s[i]);
-        }
-        const float mn = fmaxf(m, fmaxf(mx, other_half(mx)));
-        const float base = mn == -INFINITY ? 0.0f : mn - kShift;
-        const float corr = mn == -INFINITY ? 1.0f : exp2f(m - mn);
-        m = mn;
-        v8h ph[2], pl[2];
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float p = exp2f(s[i] - base);
-            sum += p;
-            const _Float16 hp = (_Float16)p;
-            ph[i >> 3][i & 7] = hp;
-            pl[i >> 3][i & 7] = (_Float16)(p - (float)hp);
-        }
-        l = l * corr + sum;
-#pragma unroll
-        for (int et = 0; et < ET; et++) {
+        for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                o[et][i] *= corr;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[et][u], ph[u], o[et], 0, 0, 0);
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[et][u], pl[u], o[et], 0, 0, 0);
-            }
-        }
-    }
-    // the wavefronts' parts, in their order
-    l += other_half(l);
-    if (h == 0) {
-        ms[wave][li] = m;
-        ls[wave][li] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++)
-        top = fmaxf(top, ms[w][li]);
-    const float corr = m == -INFINITY ? 0.0f : exp2f(m - top);
-    for (int w = 0; w < kWaves; w++) {
-        if (wave == w) {
+                mx = fmaxf(mx, s[u][i]);
+        mx = fmaxf(mx, other_half(mx));
+        // (a row that sees nothing yet, or whose maximum has risen past what the
+        // reference allows: the reference becomes the maximum)
+        if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
+            const float mn = fmaxf(m, mx);
+            const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+            m = mn;
+            l *= corr;
 #pragma unroll
             for (int et = 0; et < ET; et++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float *to = &os[li][32 * et + 8 * (i >> 2) + 4 * h + (i & 3)];
-                    const float v = m == -INFINITY ? 0.0f : o[et][i] * corr;
-                    *to = w == 0 ? v : *to + v;
-                }
+                for (int i = 0; i < 16; i++)
+                    o[et][i] *= corr;
         }
-        __syncthreads();
-    }
-    for (int i = tid; i < kTile * HD; i += 64 * kWaves) {
-        const int rr = i / HD, e = i - rr * HD;
-        if (r0 + rr < R) {
-            const int nd = (r0 + rr) / g, hh = kvh * g + (r0 + rr - nd * g);
-            x.po[(((size_t)sp * x.M + t.f0 + nd) * x.heads + hh) * HD + e] = os[rr][e];
-        }
-    }
-    if (tid < kTile && r0 + tid < R) {
-        float sum = 0.0f;
+        const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
+        v8h ph[4], pl[4];
 #pragma unroll
-        for (int w = 0; w < kWaves; w++)
-            sum += ms[w][tid] == -INFINITY ? ls[w][tid] : ls[w][tid] * exp2f(ms[w][tid] - top);
-        const int nd = (r0 + tid) / g, hh = kvh * g + (r0 + tid - nd * g);
-        float *to = x.pml + (((size_t)sp * x.M + t.f0 + nd) * x.heads + hh) * 2;
-        to[0] = top;
-        to[1] = sum;
+        for (int w = 0; w < 4; w++) {
+            uint32_t hb[4], lb[4];
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[w >> 1][8 * (w & 1) + 2 * i], x.c, base));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[w >> 1][8 * (w & 1) + 2 * i + 1], x.c, base));
+                part += p + p1;
+                hb[i] = pack_rtz(p, p1);
+                lb[i] = pack_rtz(fmaf(half_bits_to_float(hb[i]), -1.0f, p), fmaf(half_bits_to_float(hb[i] >> 16), -1.0f, p1));
+            }
+            l += part;
+            const v4u hv = {hb[0], hb[1], hb[2], hb[3]}, lv = {lb[0], lb[1], lb[2], lb[3]};
+            ph[w] = __builtin_bit_cast(v8h, hv);
+            pl[w] = __builtin_bit_cast(v8h, lv);
+        }
+#pragma unroll
+        for (int et = 0; et < ET; et++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const v8h v = *(const v8h *)(st + vlane + 4096 * et + (((uint32_t)(2 * w) ^ vx) << 4));
+                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[w], o[et], 0, 0, 0);
+                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[w], o[et], 0, 0, 0);
+            }
+    }
+    if (r0 + li >= R)
+        return;
+    l += other_half(l);
+    const size_t row = ((size_t)sp * x.M + t.f0 + node) * x.heads + kvh * g + (r - node * g);
+    float *po = x.po + row * HD + 4 * h;
+#pragma unroll
+    for (int et = 0; et < ET; et++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const v4f w = {o[et][4 * i], o[et][4 * i + 1], o[et][4 * i + 2], o[et][4 * i + 3]};
+            *(v4f *)(po + 32 * et + 8 * i) = w;
+        }
+    if (h == 0) {
+        x.pml[2 * row] = m == -INFINITY ? m : m * x.c;
+        x.pml[2 * row + 1] = l;
     }
 }
 
@@ -299,20 +344,29 @@ __global__ __launch_bounds__(64) void attn_tree_join_kernel(const Args x, float 
     }
 }
 
-// Workgroups for two rounds of the CUs, each share at least eight steps a
-// wavefront.
+// Wavefronts a workgroup: a group's tiles of rows, the groups alike.
+struct Groups {
+    int waves, groups;
+    Groups(int max_nodes, int heads, int kv_heads) {
+        const int tiles = (max_nodes * (heads / kv_heads) + kTile - 1) / kTile;
+        groups = (tiles + kMaxWaves - 1) / kMaxWaves;
+        waves = (tiles + groups - 1) / groups;
+    }
+};
+
+// Shares of the keys: about a workgroup a CU.
 int splits(int n, int max_nodes, int heads, int kv_heads, int max_prefix) {
-    const int tiles = (max_nodes * (heads / kv_heads) + kTile - 1) / kTile;
-    const int steps = (max_prefix + kTile - 1) / kTile + (max_nodes + 7 + kTile - 1) / kTile;
-    const int most = std::max(1, steps / (4 * kWaves));
-    return (int)std::max<int64_t>(1, std::min<int64_t>({most, kMaxSplits, 1024 / ((int64_t)std::max(n, 1) * kv_heads * tiles) + 1}));
+    const Groups w(max_nodes, heads, kv_heads);
+    const int steps = (max_prefix + kStage - 1) / kStage + (max_nodes + 7 + kStage - 1) / kStage;
+    const int64_t one = (int64_t)std::max(n, 1) * kv_heads * w.groups;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, (512 / w.waves + 256) / one}));
 }
 
 template <int HD>
 int launch_hd(gx_ctx *ctx, const Args &x, float *out, int8_t *q, float *scales, int32_t *qsum) {
-    const int tiles = (x.max_nodes * (x.heads / x.kv_heads) + kTile - 1) / kTile;
-    const dim3 grid((unsigned)x.kv_heads, (unsigned)tiles, (unsigned)(x.n * x.S));
-    attn_tree_kernel<HD><<<grid, 64 * kWaves, 0, ctx->stream>>>(x);
+    const Groups w(x.max_nodes, x.heads, x.kv_heads);
+    const dim3 grid((unsigned)x.kv_heads, (unsigned)w.groups, (unsigned)(x.n * x.S));
+    attn_tree_kernel<HD><<<grid, 64 * w.waves, 2 * 256 * HD, ctx->stream>>>(x);
     if (int rc = check_launch("attention of drafted trees"))
         return rc;
     const dim3 join((unsigned)((x.heads * HD + 63) / 64), (unsigned)x.M);
