@@ -148,6 +148,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const uint32_t klane = h * 1024 + ((li & ~12) | ((li & 4) << 1) | ((li & 8) >> 1)) * 16;
     const uint32_t vlane = HD * 128 + li * 128, vx = h ^ (li & 7);
 
+    // the first four wavefronts go first: the others' matrix products then run
+    // beside their exponentials
+    if (wave < 4)
+        __builtin_amdgcn_s_setprio(1);
     v16f o[ET] = {};
     float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
     int at = 0;
@@ -265,17 +269,46 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     }
 }
 
-// One head element a lane: the shares of a row joined in order, and the Q8_0
-// of 32 elements.  grid (heads * HD / 64, M), 64 threads.
-//
-// An infinite or NaN value that a row's mask hides still makes 0 * inf in its
-// tile: a row whose sum is a number and whose output is none is computed
-// again here, key by key over what it sees alone.
+// The value at row `row` of the rows a node sees of an element that a masked
+// value has spoilt, key by key: an infinite or NaN value that the mask hides
+// makes 0 * inf in its step.
 template <int HD>
-__global__ __launch_bounds__(64) void attn_tree_join_kernel(const Args x, float *__restrict__ out,
-                                                            int8_t *__restrict__ q8, float *__restrict__ scales,
-                                                            int32_t *__restrict__ qsum) {
-    const int lane = threadIdx.x, tok = blockIdx.y, width = x.heads * HD;
+__device__ float attn_tree_again(const Args &x, const Tree &t, int b, int tok, int head, int e, float top) {
+    const int kvh = head / (x.heads / x.kv_heads);
+    const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
+    const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
+    const uint16_t *qr = x.qh + ((size_t)tok * x.heads + head) * HD;
+    const uint32_t *mrow = x.mask + (size_t)tok * x.words;
+    float o = 0.0f;
+    for (int part = 0; part < 2; part++) {
+        const int rows = part ? x.draft_context : x.context, base = part ? t.f0 : 0, count = part ? t.T : t.P;
+        const uint16_t *kb = part ? x.kd + (size_t)kvh * HD * rows : x.kc + cache;
+        const uint16_t *vb = (part ? x.vd + (size_t)kvh * HD * rows : x.vc + cache) + (size_t)e * rows + base;
+        for (int j = 0; j < count; j++) {
+            if (part && !(mrow[j >> 5] >> (j & 31) & 1))
+                continue;
+            float s = 0.0f;
+            for (int k = 0; k < HD; k++)
+                s = fmaf(half_bits_to_float(qr[k]), half_bits_to_float(kb[((size_t)(k >> 3) * rows + base + j) * 8 + (k & 7)]),
+                         s);
+            o = fmaf(exp2f(s * x.c - top + kShift), half_bits_to_float(vb[j]), o);
+        }
+    }
+    return o;
+}
+
+// A row (a node's head) a wavefront: its shares' maxima and sums a lane each,
+// its outputs four elements a lane, several shares side by side, added in a
+// fixed order; and the Q8_0 of 32 elements.  grid (heads / 4, M), 256 threads.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float *__restrict__ out,
+                                                             int8_t *__restrict__ q8, float *__restrict__ scales,
+                                                             int32_t *__restrict__ qsum) {
+    constexpr int L = HD / 4, SP = 64 / L;  // lanes a share, shares side by side
+    const int lane = threadIdx.x & 63, tok = blockIdx.y, width = x.heads * HD;
+    const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (head >= x.heads)
+        return;
     int b = 0, hi = x.n;  // the tree: the last whose first token is not past this one
     while (hi - b > 1) {
         const int mid = (b + hi) >> 1;
@@ -287,59 +320,65 @@ __global__ __launch_bounds__(64) void attn_tree_join_kernel(const Args x, float 
     const Tree t(x, b);
     if (tok < t.f0 || tok >= t.f0 + t.T)
         return;
-    const int col = min((int)blockIdx.x * 64 + lane, width - 1), head = col / HD, e = col - head * HD;
-    const int live = (t.total + t.per - 1) / t.per;
+    const int live = (t.total + t.per - 1) / t.per;  // at most 64
     const size_t row = (size_t)tok * x.heads + head, step = (size_t)x.M * x.heads;
-    float top = -INFINITY;
-    for (int s = 0; s < live; s++)
-        top = fmaxf(top, x.pml[(s * step + row) * 2]);
-    float l = 0.0f, o = 0.0f;
-    for (int s = 0; s < live; s++) {
-        const float m = x.pml[(s * step + row) * 2];
-        const float corr = m == -INFINITY ? (top == -INFINITY ? 1.0f : 0.0f) : exp2f(m - top);
-        const float sl = x.pml[(s * step + row) * 2 + 1], so = x.po[(s * step + row) * HD + e];
-        l += m == -INFINITY ? sl : sl * corr;
-        o += m == -INFINITY ? 0.0f : so * corr;
-    }
+    const int g = lane / L, e = 4 * (lane - g * L);
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    const v2f ml = *(const v2f *)(x.pml + (min(lane, live - 1) * step + row) * 2);
+    const float *po = x.po + row * HD + e;
     const uint32_t *mrow = x.mask + (size_t)tok * x.words;
-    bool any = t.P > 0;
-    for (int w = 0; 32 * w < t.T; w++)
-        any |= (mrow[w] & (t.T - 32 * w >= 32 ? ~0u : (1u << (t.T - 32 * w)) - 1)) != 0;
-    if (any && l - l == 0.0f && o - o != 0.0f) {
-        const int g = x.heads / x.kv_heads, kvh = head / g;
-        const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
-        const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
-        const uint16_t *qr = x.qh + row * HD;
-        o = 0.0f;
-        for (int part = 0; part < 2; part++) {
-            const int rows = part ? x.draft_context : x.context, base = part ? t.f0 : 0, count = part ? t.T : t.P;
-            const uint16_t *kb = part ? x.kd + (size_t)kvh * HD * rows : x.kc + cache;
-            const uint16_t *vb = (part ? x.vd + (size_t)kvh * HD * rows : x.vc + cache) + (size_t)e * rows + base;
-            for (int j = 0; j < count; j++) {
-                if (part && !(mrow[j >> 5] >> (j & 31) & 1))
-                    continue;
-                float s = 0.0f;
-                for (int k = 0; k < HD; k++)
-                    s = fmaf(half_bits_to_float(qr[k]),
-                             half_bits_to_float(kb[((size_t)(k >> 3) * rows + base + j) * 8 + (k & 7)]), s);
-                o = fmaf(exp2f(s * x.c - top + kShift), half_bits_to_float(vb[j]), o);
-            }
+    const int bits = t.T - 32 * lane;  // nodes that this lane's mask word speaks of
+    const uint32_t word = bits > 0 ? mrow[lane] & (bits >= 32 ? ~0u : (1u << bits) - 1) : 0u;
+    const bool any = t.P > 0 || __ballot(word != 0) != 0;
+    const float m = lane < live ? ml.x : -INFINITY, top = wave_max(m);
+    const float weight = m == -INFINITY ? 0.0f : exp2f(m - top);
+    // (a share that saw nothing, or nothing but NaN, has no maximum)
+    const float l = wave_pairwise_sum(lane < live ? (m == -INFINITY ? ml.y : ml.y * weight) : 0.0f);
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < live; s0 += 4 * SP) {
+        v4f p[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            p[k] = *(const v4f *)(po + (size_t)min(s0 + k * SP + g, live - 1) * step * HD);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int s = s0 + k * SP + g;
+            const float w = __shfl(weight, s & 63);
+            if (s < live && w != 0.0f && g < SP)
+                o += p[k] * w;
         }
     }
-    const float y = any ? o / l : 0.0f;
-    const bool in = (int)blockIdx.x * 64 + lane < width;
-    if (out && in)
-        out[(size_t)tok * width + col] = y;
+    for (int k = 1; k < SP; k++) {
+        v4f p;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            p[i] = __shfl(o[i], (lane + k * L) & 63);
+        if (lane < L)
+            o += p;
+    }
+    if (lane >= L)
+        return;
+    v4f y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (any && l - l == 0.0f && o[i] - o[i] != 0.0f)
+            o[i] = attn_tree_again<HD>(x, t, b, tok, head, e + i, top);
+        y[i] = any ? o[i] / l : 0.0f;
+    }
+    const size_t at = (size_t)tok * width + head * HD + e;
+    if (out)
+        for (int i = 0; i < 4; i++)
+            out[at + i] = y[i];
     if (q8) {
+        const float v[4] = {y[0], y[1], y[2], y[3]};
         float stored;
         int32_t sm;
-        const int32_t nq = q8_0_lane(in ? y : 0.0f, &stored, &sm);
-        if (in) {
-            q8[(size_t)tok * width + col] = (int8_t)nq;
-            if ((lane & 31) == 0) {
-                scales[(size_t)tok * (width >> 5) + (col >> 5)] = stored;
-                qsum[(size_t)tok * (width >> 5) + (col >> 5)] = sm;
-            }
+        const uint32_t packed = q8_0_quad(v, &stored, &sm);
+        for (int i = 0; i < 4; i++)
+            q8[at + i] = (int8_t)(packed >> (8 * i));
+        if ((lane & 7) == 0) {
+            scales[at >> 5] = stored;
+            qsum[at >> 5] = sm;
         }
     }
 }
@@ -354,12 +393,14 @@ struct Groups {
     }
 };
 
-// Shares of the keys: about a workgroup a CU.
+// Shares of the keys: as many workgroups as run at once (two wavefronts a SIMD
+// by their registers, two workgroups a CU by their LDS), so that the last round
+// is whole.
 int splits(int n, int max_nodes, int heads, int kv_heads, int max_prefix) {
     const Groups w(max_nodes, heads, kv_heads);
     const int steps = (max_prefix + kStage - 1) / kStage + (max_nodes + 7 + kStage - 1) / kStage;
-    const int64_t one = (int64_t)std::max(n, 1) * kv_heads * w.groups;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, (512 / w.waves + 256) / one}));
+    const int64_t one = (int64_t)std::max(n, 1) * kv_heads * w.groups, most = w.waves > 4 ? 256 : 512;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, most / one}));
 }
 
 template <int HD>
@@ -369,8 +410,8 @@ int launch_hd(gx_ctx *ctx, const Args &x, float *out, int8_t *q, float *scales, 
     attn_tree_kernel<HD><<<grid, 64 * w.waves, 2 * 256 * HD, ctx->stream>>>(x);
     if (int rc = check_launch("attention of drafted trees"))
         return rc;
-    const dim3 join((unsigned)((x.heads * HD + 63) / 64), (unsigned)x.M);
-    attn_tree_join_kernel<HD><<<join, 64, 0, ctx->stream>>>(x, out, q, scales, qsum);
+    const dim3 join((unsigned)((x.heads + 3) / 4), (unsigned)x.M);
+    attn_tree_join_kernel<HD><<<join, 256, 0, ctx->stream>>>(x, out, q, scales, qsum);
     return check_launch("attention of drafted trees, joined");
 }
 
