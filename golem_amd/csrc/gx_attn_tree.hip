@@ -68,7 +68,13 @@ struct Tree {
     }
 };
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// The larger of a lane's value and the other half's.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// LDS reads asked for before this are asked for here, not where they are used.
+__device__ __forceinline__ void reads_first() { asm volatile("" ::: "memory"); }
 
 // Elements lo .. hi - 1 of eight, the rest zero.
 __device__ __forceinline__ v8h keep(v8h v, int lo, int hi) {
@@ -76,6 +82,18 @@ __device__ __forceinline__ v8h keep(v8h v, int lo, int hi) {
 #pragma unroll
     for (int j = 0; j < 8; j++)
         r[j] = j >= lo && j < hi ? v[j] : (_Float16)0.0f;
+    return r;
+}
+
+// lo/hi(a) * lo/hi(b) + c for fp16 pairs a and b, as one v_fma_mix.
+__device__ __forceinline__ float fma_mix_lo(uint32_t a, uint32_t b, float c) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,1,0]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float fma_mix_hi(uint32_t a, uint32_t b, float c) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
 
@@ -175,14 +193,28 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         }
         if (r0 >= R)
             continue;
+        v8h a[KS][2];
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                a[k][u] = *(const v8h *)(st + klane + 2048 * k + 512 * u);
+        reads_first();
         v16f s[2] = {};
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const v8h a = *(const v8h *)(st + klane + 2048 * k + 512 * u);
-                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[k], s[u], 0, 0, 0);
-            }
+            for (int u = 0; u < 2; u++)
+                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k][u], q[k], s[u], 0, 0, 0);
+        v8h v[4][ET];
+        auto values = [&](int w) __attribute__((always_inline)) {
+#pragma unroll
+            for (int et = 0; et < ET; et++)
+                v[w][et] = *(const v8h *)(st + vlane + 4096 * et + (((uint32_t)(2 * w) ^ vx) << 4));
+        };
+        values(0);
+        values(1);
+        reads_first();
         if (draft || p0 + kStage > hi) {
             uint32_t sees[2] = {~0u, ~0u};
             if (draft) {
@@ -209,7 +241,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
 #pragma unroll
             for (int i = 0; i < 16; i++)
                 mx = fmaxf(mx, s[u][i]);
-        mx = fmaxf(mx, other_half(mx));
+        mx = halves_max(mx);
         // (a row that sees nothing yet, or whose maximum has risen past what the
         // reference allows: the reference becomes the maximum)
         if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
@@ -225,8 +257,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         }
         const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
         v8h ph[4], pl[4];
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
+        auto chances = [&](int w) __attribute__((always_inline)) {
             uint32_t hb[4], lb[4];
             float part = 0.0f;
 #pragma unroll
@@ -235,25 +266,31 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(s[w >> 1][8 * (w & 1) + 2 * i + 1], x.c, base));
                 part += p + p1;
                 hb[i] = pack_rtz(p, p1);
-                lb[i] = pack_rtz(fmaf(half_bits_to_float(hb[i]), -1.0f, p), fmaf(half_bits_to_float(hb[i] >> 16), -1.0f, p1));
+                lb[i] = pack_rtz(fma_mix_lo(hb[i], 0xBC00BC00u, p), fma_mix_hi(hb[i], 0xBC00BC00u, p1));
             }
             l += part;
             const v4u hv = {hb[0], hb[1], hb[2], hb[3]}, lv = {lb[0], lb[1], lb[2], lb[3]};
             ph[w] = __builtin_bit_cast(v8h, hv);
             pl[w] = __builtin_bit_cast(v8h, lv);
+        };
+        chances(0);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+#pragma unroll
+            for (int et = 0; et < ET; et++)
+                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], ph[w], o[et], 0, 0, 0);
+#pragma unroll
+            for (int et = 0; et < ET; et++)
+                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], pl[w], o[et], 0, 0, 0);
+            if (w < 2)
+                values(w + 2);
+            if (w < 3)
+                chances(w + 1);
         }
-#pragma unroll
-        for (int et = 0; et < ET; et++)
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const v8h v = *(const v8h *)(st + vlane + 4096 * et + (((uint32_t)(2 * w) ^ vx) << 4));
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[w], o[et], 0, 0, 0);
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[w], o[et], 0, 0, 0);
-            }
     }
     if (r0 + li >= R)
         return;
-    l += other_half(l);
+    l += __shfl_xor(l, 32);
     const size_t row = ((size_t)sp * x.M + t.f0 + node) * x.heads + kvh * g + (r - node * g);
     float *po = x.po + row * HD + 4 * h;
 #pragma unroll
