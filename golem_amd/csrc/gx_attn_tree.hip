@@ -58,9 +58,9 @@ struct Args {
 struct Tree {
     int f0, T, P, a, np, total, per;  // (total and per: steps)
     __device__ Tree(const Args &x, int b) {
-        f0 = min(max(x.first[b], 0), x.M);
-        T = min(min(max(x.first[b + 1], f0), x.M) - f0, x.max_nodes);
-        P = min(max(x.prefix[b], 0), min(x.max_prefix, x.context));
+        f0 = __builtin_amdgcn_readfirstlane(min(max(x.first[b], 0), x.M));
+        T = __builtin_amdgcn_readfirstlane(min(min(max(x.first[b + 1], f0), x.M) - f0, x.max_nodes));
+        P = __builtin_amdgcn_readfirstlane(min(max(x.prefix[b], 0), min(x.max_prefix, x.context)));
         a = f0 & 7;  // draft rows are read from a multiple of 8
         np = (P + kStage - 1) / kStage;
         total = np + (T > 0 ? (a + T + kStage - 1) / kStage : 0);
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
     if (g0 >= R || t0 >= t1)
         return;
-    const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
+    const int slot = __builtin_amdgcn_readfirstlane(x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0);
     const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
     const uint16_t *kc = x.kc + cache, *vc = x.vc + cache;
     const uint16_t *kd = x.kd + (size_t)kvh * HD * x.draft_context, *vd = x.vd + (size_t)kvh * HD * x.draft_context;
@@ -141,7 +141,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         const int rows = draft ? x.draft_context : x.context;
         const char *kb = (const char *)(draft ? kd : kc), *vb = (const char *)(draft ? vd : vc);
         const uint32_t kp = (uint32_t)min(max(p0 + lane, lo), hi - 1) * 16;
-        const uint32_t vp = ((uint32_t)(lane >> 3) * rows + min(p0 + 8 * ((lane & 7) ^ (lane >> 3)), rows - 8)) * 2;
+        const int pv = min(max(p0 + 8 * ((lane & 7) ^ (lane >> 3)), lo & ~7), (hi - 1) & ~7);
+        const uint32_t vp = ((uint32_t)(lane >> 3) * rows + pv) * 2;
         // (a uniform base and the lane's 32-bit offset: no vector instruction a load)
         for (int i = wave; i < HD / 8; i += nw) {
             const char *src = kb + (size_t)i * rows * 16;
@@ -163,6 +164,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     for (int s = 0; s < KS; s++)
         q[s] = *(const v8h *)(qr + 16 * s);
     const uint32_t *mrow = x.mask + (size_t)(t.f0 + node) * x.words;
+    uint32_t mw[3] = {0u, mrow[0], x.words > 1 ? mrow[1] : 0u};  // the words before, at and after a draft step's first
     const uint32_t klane = h * 1024 + ((li & ~12) | ((li & 4) << 1) | ((li & 8) >> 1)) * 16;
     const uint32_t vlane = HD * 128 + li * 128, vx = h ^ (li & 7);
 
@@ -181,12 +183,19 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         uint8_t *st = lds + at;
         int p0, lo, hi;
         const bool draft = rows_of(j, p0, lo, hi);
-        if (p0 < lo || p0 + kStage > hi) {  // rows of the step that there are not: their values become zero
-            for (int i = tid; i < HD * 8; i += 64 * nw) {
-                const int e = i >> 3, pv = p0 + 8 * ((i & 7) ^ (e & 7));
-                if (pv < lo || pv + 8 > hi) {
-                    v8h *to = (v8h *)(st + HD * 128 + i * 16);
-                    *to = keep(*to, lo - pv, hi - pv);
+        // Keys and chunks of values past the rows that there are repeat one that is
+        // (its chance will be zero); the rows beside those in a chunk become zero.
+        const int cl = p0 < lo ? (lo - p0) >> 3 : -1, ch = p0 + kStage > hi ? (hi - p0) >> 3 : -1;
+        if ((cl >= 0 && (lo & 7)) || (ch >= 0 && (hi & 7))) {
+            for (int e = tid; e < HD; e += 64 * nw) {
+                uint8_t *vr = st + HD * 128 + e * 128;
+                if (cl >= 0) {
+                    v8h *to = (v8h *)(vr + ((cl ^ (e & 7)) << 4));
+                    *to = keep(*to, lo - (p0 + 8 * cl), hi - (p0 + 8 * cl));
+                }
+                if (ch >= 0 && ch < 8) {
+                    v8h *to = (v8h *)(vr + ((ch ^ (e & 7)) << 4));
+                    *to = keep(*to, lo - (p0 + 8 * ch), hi - (p0 + 8 * ch));
                 }
             }
             lds_barrier();
@@ -216,24 +225,32 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         values(1);
         reads_first();
         if (draft || p0 + kStage > hi) {
-            uint32_t sees[2] = {~0u, ~0u};
+            // bit k of sees[u]: key 32 u + k of the step
+            const int above = hi - p0, below = max(lo - p0, 0);
+            uint32_t sees[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int n = min(max(above - 32 * u, 0), 32), z = min(max(below - 32 * u, 0), 32);
+                sees[u] = (uint32_t)((1ull << n) - (1ull << z)) & (n > z ? ~0u : 0u);
+            }
             if (draft) {
                 const int w0 = 2 * (j - t.np);  // bits from node 32 w0 - a on
-                uint32_t w[3];
+                if (w0 > 0) {
 #pragma unroll
-                for (int i = 0; i < 3; i++)
-                    w[i] = w0 + i > 0 && w0 + i <= x.words ? mrow[w0 + i - 1] : 0u;
+                    for (int i = 0; i < 3; i++)
+                        mw[i] = w0 + i <= x.words ? mrow[w0 + i - 1] : 0u;
+                }
 #pragma unroll
                 for (int u = 0; u < 2; u++)
-                    sees[u] = t.a ? (w[u + 1] << t.a) | (w[u] >> (32 - t.a)) : w[u + 1];
+                    sees[u] &= t.a ? (mw[u + 1] << t.a) | (mw[u] >> (32 - t.a)) : mw[u + 1];
             }
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++) {
+                const uint32_t bits = sees[u] >> (8 * h);
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int k = 16 * (i >> 3) + 8 * h + (i & 7), p = p0 + 32 * u + k;
-                    s[u][i] = (sees[u] >> k & 1) && p >= lo && p < hi ? s[u][i] : -INFINITY;
-                }
+                for (int i = 0; i < 16; i++)
+                    s[u][i] = bits >> (16 * (i >> 3) + (i & 7)) & 1 ? s[u][i] : -INFINITY;
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
