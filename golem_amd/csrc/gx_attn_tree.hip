@@ -323,29 +323,42 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     }
 }
 
-// The value at row `row` of the rows a node sees of an element that a masked
-// value has spoilt, key by key: an infinite or NaN value that the mask hides
-// makes 0 * inf in its step.
+// The elements of a row that a masked value has spoilt (an infinite or NaN
+// value that the mask hides makes 0 * inf in its step), summed again over what
+// the node sees alone: 64 keys at a time, a key a lane, the spoilt elements in
+// turn.  o: the row's outputs, four a lane; spoilt: which of them.
 template <int HD>
-__device__ float attn_tree_again(const Args &x, const Tree &t, int b, int tok, int head, int e, float top) {
-    const int kvh = head / (x.heads / x.kv_heads);
+__device__ __forceinline__ v4f attn_tree_again(const Args &x, const Tree &t, int b, int tok, int head, float top, v4f o,
+                                            uint32_t spoilt) {
+    const int lane = threadIdx.x & 63, kvh = head / (x.heads / x.kv_heads);
     const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
     const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
     const uint16_t *qr = x.qh + ((size_t)tok * x.heads + head) * HD;
     const uint32_t *mrow = x.mask + (size_t)tok * x.words;
-    float o = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        o[i] = spoilt >> i & 1 ? 0.0f : o[i];
     for (int part = 0; part < 2; part++) {
         const int rows = part ? x.draft_context : x.context, base = part ? t.f0 : 0, count = part ? t.T : t.P;
         const uint16_t *kb = part ? x.kd + (size_t)kvh * HD * rows : x.kc + cache;
-        const uint16_t *vb = (part ? x.vd + (size_t)kvh * HD * rows : x.vc + cache) + (size_t)e * rows + base;
-        for (int j = 0; j < count; j++) {
-            if (part && !(mrow[j >> 5] >> (j & 31) & 1))
-                continue;
+        const uint16_t *vb = part ? x.vd + (size_t)kvh * HD * rows : x.vc + cache;
+        for (int j0 = 0; j0 < count; j0 += 64) {
+            const int j = min(j0 + lane, count - 1);
+            const bool sees = j0 + lane < count && (!part || (mrow[j >> 5] >> (j & 31) & 1));
             float s = 0.0f;
             for (int k = 0; k < HD; k++)
                 s = fmaf(half_bits_to_float(qr[k]), half_bits_to_float(kb[((size_t)(k >> 3) * rows + base + j) * 8 + (k & 7)]),
                          s);
-            o = fmaf(exp2f(s * x.c - top + kShift), half_bits_to_float(vb[j]), o);
+            const float p = exp2f(s * x.c - top + kShift);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                for (unsigned long long who = __ballot(spoilt >> i & 1); who; who &= who - 1) {
+                    const int l = __builtin_ctzll(who);
+                    const float v = half_bits_to_float(vb[(size_t)(4 * l + i) * rows + base + j]);
+                    const float sum = wave_pairwise_sum(sees ? p * v : 0.0f);
+                    if (lane == l)
+                        o[i] += sum;
+                }
         }
     }
     return o;
@@ -363,16 +376,11 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
     const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head >= x.heads)
         return;
-    int b = 0, hi = x.n;  // the tree: the last whose first token is not past this one
-    while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (x.first[mid] <= tok)
-            b = mid;
-        else
-            hi = mid;
-    }
-    const Tree t(x, b);
-    if (tok < t.f0 || tok >= t.f0 + t.T)
+    int b = -1;  // the tree: the last whose first token is not past this one
+    for (int i = 0; i < x.n; i += 64)
+        b += __popcll(__ballot(i + lane < x.n && x.first[min(i + lane, x.n - 1)] <= tok));
+    const Tree t(x, max(b, 0));
+    if (b < 0 || tok < t.f0 || tok >= t.f0 + t.T)
         return;
     const int live = (t.total + t.per - 1) / t.per;  // at most 64
     const size_t row = (size_t)tok * x.heads + head, step = (size_t)x.M * x.heads;
@@ -380,9 +388,17 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
     typedef float v2f __attribute__((ext_vector_type(2)));
     const v2f ml = *(const v2f *)(x.pml + (min(lane, live - 1) * step + row) * 2);
     const float *po = x.po + row * HD + e;
+    auto shares = [&](int s0, v4f *p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            p[k] = *(const v4f *)(po + (size_t)min(s0 + k * SP + g, live - 1) * step * HD);
+    };
+    v4f p[4];
+    shares(0, p);
     const uint32_t *mrow = x.mask + (size_t)tok * x.words;
     const int bits = t.T - 32 * lane;  // nodes that this lane's mask word speaks of
     const uint32_t word = bits > 0 ? mrow[lane] & (bits >= 32 ? ~0u : (1u << bits) - 1) : 0u;
+    reads_first();
     const bool any = t.P > 0 || __ballot(word != 0) != 0;
     const float m = lane < live ? ml.x : -INFINITY, top = wave_max(m);
     const float weight = m == -INFINITY ? 0.0f : exp2f(m - top);
@@ -390,10 +406,8 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
     const float l = wave_pairwise_sum(lane < live ? (m == -INFINITY ? ml.y : ml.y * weight) : 0.0f);
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < live; s0 += 4 * SP) {
-        v4f p[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            p[k] = *(const v4f *)(po + (size_t)min(s0 + k * SP + g, live - 1) * step * HD);
+        if (s0 > 0)
+            shares(s0, p);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int s = s0 + k * SP + g;
@@ -410,15 +424,19 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
         if (lane < L)
             o += p;
     }
+    uint32_t spoilt = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (lane < L && any && l - l == 0.0f && o[i] - o[i] != 0.0f)
+            spoilt |= 1u << i;
+    if (__ballot(spoilt != 0))
+        o = attn_tree_again<HD>(x, t, b, tok, head, top, o, spoilt);
     if (lane >= L)
         return;
     v4f y;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (any && l - l == 0.0f && o[i] - o[i] != 0.0f)
-            o[i] = attn_tree_again<HD>(x, t, b, tok, head, e + i, top);
+    for (int i = 0; i < 4; i++)
         y[i] = any ? o[i] / l : 0.0f;
-    }
     const size_t at = (size_t)tok * width + head * HD + e;
     if (out)
         for (int i = 0; i < 4; i++)
