@@ -12,82 +12,146 @@ namespace {
 // a node's bits hold its first 2^k ancestors, itself included, `up` is the
 // next one above them, and depth counts them; nine rounds reach 512.  A node
 // whose parent is no earlier node has no place, and so have the nodes below.
-// grid n + 1: a workgroup a tree, the last one for the tokens behind the trees.
+// A tree of at most 64 nodes is a wavefront's: a lane a node, two words of bits,
+// a step up one exchange; larger ones take the workgroup and LDS.
+// grid (n + 1, pieces): workgroups a tree, each with every pieces-th of the
+// rotation rows; the last tree stands for the tokens behind the trees.
 constexpr int kPlanThreads = 256;
 
 __global__ __launch_bounds__(kPlanThreads) void tree_plan_kernel(
     int n, int M, int max_nodes, int words, const int32_t *__restrict__ first, const int32_t *__restrict__ parents,
     const int32_t *__restrict__ prefix, const float *__restrict__ rope_cos, const float *__restrict__ rope_sin,
-    int half, int context, int32_t *__restrict__ rows, int32_t *__restrict__ positions, uint32_t *__restrict__ mask,
-    float *__restrict__ cos, float *__restrict__ sin) {
+    int half, int context, bool wide, int32_t *__restrict__ rows, int32_t *__restrict__ positions,
+    uint32_t *__restrict__ mask, float *__restrict__ cos, float *__restrict__ sin) {
     constexpr int kMine = kTreeNodes / kPlanThreads;
     constexpr int kBits = kTreeNodes * (kTreeNodes / 32) / kPlanThreads;
     __shared__ uint32_t bits[kTreeNodes * (kTreeNodes / 32)];
     __shared__ int16_t up[kTreeNodes], depth[kTreeNodes];  // up: -1 above a root, -2 no place
     __shared__ int place[kTreeNodes];                      // a node's position, or -1
-    const int tid = threadIdx.x, b = blockIdx.x;
-    const bool tail = b == n;
+    const int tid = threadIdx.x, b = blockIdx.x, lane = tid & 63;
+    const bool tail = b == n, writes = blockIdx.y == 0;
     const int f0 = min(max(first[tail ? n : b], 0), M), f1 = tail ? M : min(max(first[b + 1], f0), M);
     const int T = tail ? 0 : min(f1 - f0, max_nodes);
-    for (int i = tid; i < T; i += kPlanThreads) {
-        const int p = parents[f0 + i];
-        up[i] = (int16_t)(p == -1 ? -1 : p >= 0 && p < i ? p : -2);
-        depth[i] = 1;
-    }
-    for (int i = tid; i < T * words; i += kPlanThreads) {
-        const int node = i / words, w = i - node * words;
-        bits[i] = node >> 5 == w ? 1u << (node & 31) : 0u;
-    }
-    __syncthreads();
-    for (int span = 1; span < T; span <<= 1) {
-        int16_t u[kMine], d[kMine];
-        uint32_t w[kBits];
-#pragma unroll
-        for (int k = 0; k < kMine; k++) {
-            const int i = tid + k * kPlanThreads;
-            if (i < T) {
-                u[k] = up[i] < 0 ? up[i] : up[up[i]];
-                d[k] = up[i] < 0 ? depth[i] : (int16_t)(depth[i] + depth[up[i]]);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kBits; k++) {
-            const int i = tid + k * kPlanThreads;
-            if (i < T * words) {
-                const int node = i / words;
-                w[k] = bits[i] | (up[node] < 0 ? 0u : bits[up[node] * words + i - node * words]);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kMine; k++) {
-            const int i = tid + k * kPlanThreads;
-            if (i < T) {
-                up[i] = u[k];
-                depth[i] = d[k];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kBits; k++) {
-            const int i = tid + k * kPlanThreads;
-            if (i < T * words)
-                bits[i] = w[k];
-        }
-        __syncthreads();
-    }
     const int base = tail ? -1 : prefix[b];
-    for (int i = tid; i < f1 - f0; i += kPlanThreads) {
-        const int64_t p = i < T && up[i] == -1 && base >= 0 ? (int64_t)base + depth[i] - 1 : -1;
-        const int at = p < context ? (int)p : -1;
-        if (i < T)
-            place[i] = at;
-        rows[f0 + i] = at < 0 ? -1 : f0 + i;
-        positions[f0 + i] = at;
+    if (T <= 64) {
+        if (tid < 64) {
+            const int p = lane < T ? parents[f0 + lane] : -2;
+            int u = p == -1 ? -1 : p >= 0 && p < lane ? p : -2, d = 1;
+            uint32_t w0 = lane < 32 ? 1u << lane : 0u, w1 = lane < 32 ? 0u : 1u << (lane - 32);
+            for (int span = 1; span < T; span <<= 1) {
+                const int at = max(u, 0), uu = __shfl(u, at), dd = __shfl(d, at);
+                const uint32_t x0 = __shfl(w0, at), x1 = __shfl(w1, at);
+                if (u >= 0) {
+                    u = uu;
+                    d += dd;
+                    w0 |= x0;
+                    w1 |= x1;
+                }
+            }
+            const int64_t at = u == -1 && base >= 0 ? (int64_t)base + d - 1 : -1;
+            const int pos = at < context ? (int)at : -1;
+            place[lane] = lane < T ? pos : -1;
+            if (lane < T && writes) {
+                rows[f0 + lane] = pos < 0 ? -1 : f0 + lane;
+                positions[f0 + lane] = pos;
+                uint32_t *to = mask + (size_t)(f0 + lane) * words;
+                for (int w = 0; w < words; w++)
+                    to[w] = pos < 0 || w > 1 ? 0u : w ? w1 : w0;
+            }
+        }
+        __syncthreads();
+    } else {
+        for (int i = tid; i < T; i += kPlanThreads) {
+            const int p = parents[f0 + i];
+            up[i] = (int16_t)(p == -1 ? -1 : p >= 0 && p < i ? p : -2);
+            depth[i] = 1;
+        }
+        for (int i = tid; i < T * words; i += kPlanThreads) {
+            const int node = i / words, w = i - node * words;
+            bits[i] = node >> 5 == w ? 1u << (node & 31) : 0u;
+        }
+        __syncthreads();
+        for (int span = 1; span < T; span <<= 1) {
+            int16_t u[kMine], d[kMine];
+            uint32_t w[kBits];
+#pragma unroll
+            for (int k = 0; k < kMine; k++) {
+                const int i = tid + k * kPlanThreads;
+                if (i < T) {
+                    u[k] = up[i] < 0 ? up[i] : up[up[i]];
+                    d[k] = up[i] < 0 ? depth[i] : (int16_t)(depth[i] + depth[up[i]]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kBits; k++) {
+                const int i = tid + k * kPlanThreads;
+                if (i < T * words) {
+                    const int node = i / words;
+                    w[k] = bits[i] | (up[node] < 0 ? 0u : bits[up[node] * words + i - node * words]);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kMine; k++) {
+                const int i = tid + k * kPlanThreads;
+                if (i < T) {
+                    up[i] = u[k];
+                    depth[i] = d[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kBits; k++) {
+                const int i = tid + k * kPlanThreads;
+                if (i < T * words)
+                    bits[i] = w[k];
+            }
+            __syncthreads();
+        }
+        for (int i = tid; i < T; i += kPlanThreads) {
+            const int64_t at = up[i] == -1 && base >= 0 ? (int64_t)base + depth[i] - 1 : -1;
+            const int pos = at < context ? (int)at : -1;
+            place[i] = pos;
+            if (writes) {
+                rows[f0 + i] = pos < 0 ? -1 : f0 + i;
+                positions[f0 + i] = pos;
+            }
+        }
+        __syncthreads();
+        if (writes)
+            for (int i = tid; i < T * words; i += kPlanThreads)
+                mask[(size_t)f0 * words + i] = place[i / words] >= 0 ? bits[i] : 0u;
     }
-    __syncthreads();
-    for (int i = tid; i < (f1 - f0) * words; i += kPlanThreads)
-        mask[(size_t)f0 * words + i] = i < T * words && place[i / words] >= 0 ? bits[i] : 0u;
-    for (int i = tid; i < (f1 - f0) * half; i += kPlanThreads) {
+    if (writes)  // the tokens past a tree's nodes, or past every tree
+        for (int i = T + tid; i < f1 - f0; i += kPlanThreads) {
+            rows[f0 + i] = positions[f0 + i] = -1;
+            for (int w = 0; w < words; w++)
+                mask[(size_t)(f0 + i) * words + w] = 0u;
+        }
+    const int start = blockIdx.y * kPlanThreads + tid, step = gridDim.y * kPlanThreads;
+    if (wide) {  // 16 bytes at a time
+        typedef float v4f __attribute__((ext_vector_type(4)));
+        const int pieces = half >> 2, items = (f1 - f0) * pieces;
+        for (int i0 = start; i0 < items; i0 += 2 * step) {
+            v4f c[2], s[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int i = min(i0 + u * step, items - 1), node = i / pieces, at = node < T ? place[node] : -1;
+                const size_t src = (size_t)max(at, 0) * half + 4 * (i - node * pieces);
+                c[u] = *(const v4f *)(rope_cos + src);
+                s[u] = *(const v4f *)(rope_sin + src);
+                if (at < 0)
+                    c[u] = s[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (i0 + u * step < items) {
+                    *((v4f *)(cos + (size_t)f0 * half) + i0 + u * step) = c[u];
+                    *((v4f *)(sin + (size_t)f0 * half) + i0 + u * step) = s[u];
+                }
+        }
+        return;
+    }
+    for (int i = start; i < (f1 - f0) * half; i += step) {
         const int node = i / half, k = i - node * half, at = node < T ? place[node] : -1;
         cos[(size_t)f0 * half + i] = at < 0 ? 0.0f : rope_cos[(size_t)at * half + k];
         sin[(size_t)f0 * half + i] = at < 0 ? 0.0f : rope_sin[(size_t)at * half + k];
@@ -269,6 +333,50 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
             share[b].claim = 0;
 }
 
+// grid (chunks, M): a chunk's largest logit and the lowest index that has it, by
+// gx_argmax's rule (a NaN never wins here; one at index 0 is the walk's affair).
+__global__ __launch_bounds__(kStatThreads) void verify_best_kernel(const float *__restrict__ logits, int ldl,
+                                                                   int vocab, float *__restrict__ tops,
+                                                                   int32_t *__restrict__ ids) {
+    constexpr int kMine = kStatChunk / kStatThreads;
+    __shared__ float wt[kStatThreads / 64];
+    __shared__ int wi[kStatThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.y, c0 = blockIdx.x * kStatChunk;
+    const float *x = logits + (size_t)row * ldl;
+    float v[kMine], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMine; k++) {
+        const int i = c0 + tid + k * kStatThreads;
+        const float w = x[min(i, vocab - 1)];
+        v[k] = i < vocab ? w : -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < kMine; k++)
+        top = fmaxf(top, v[k]);
+    top = wave_max(top);
+    if (lane == 0)
+        wt[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kStatThreads / 64; w++)
+        top = fmaxf(top, wt[w]);
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int k = kMine - 1; k >= 0; k--)
+        at = v[k] == top ? c0 + tid + k * kStatThreads : at;
+    at = wave_min_i32(at);
+    if (lane == 0)
+        wi[wave] = at;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kStatThreads / 64; w++)
+            at = min(at, wi[w]);
+        tops[(size_t)row * gridDim.x + blockIdx.x] = top;
+        ids[(size_t)row * gridDim.x + blockIdx.x] = at;
+    }
+}
+
 struct WalkArgs {
     const float *logits, *draft, *uniforms;
     int ldl, ldd, M, max_nodes, vocab, chunks, groups;
@@ -447,9 +555,27 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     if (tid == 0)
         path[0] = 0;
     int v = 0, kept = 1;
-    if (a.picks) {  // greedy
+    if (a.picks) {  // greedy: each row's best chunk, a wavefront a row
+        for (int i = wave; i < T; i += kWalkThreads / 64) {
+            const size_t row = f0 + i;
+            float best = -INFINITY;
+            int id = 0;
+            for (int c = lane; c < a.chunks; c += 64) {
+                const float v = a.tops[row * a.chunks + c];
+                if (v > best) {
+                    best = v;
+                    id = a.picks[row * a.chunks + c];
+                }
+            }
+            const float mx = wave_max(best);
+            id = wave_min_i32(best == mx && mx > -INFINITY ? id : 0x7fffffff);
+            const float zero = a.logits[row * a.ldl];
+            if (lane == 0)
+                gone[i] = zero != zero || id == 0x7fffffff ? 0 : id;
+        }
+        __syncthreads();
         for (int m = 1; m < T; m++)
-            if (par[m] == v && tok[m] == a.picks[f0 + v]) {
+            if (par[m] == v && tok[m] == gone[v]) {
                 if (tid == 0)
                     path[kept] = m;
                 v = m;
@@ -457,7 +583,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             }
         if (tid == 0) {
             a.counts[b] = kept;
-            a.next[b] = a.picks[f0 + v];
+            a.next[b] = gone[v];
         }
         return;
     }
@@ -738,16 +864,23 @@ int stat_chunks(int vocab) { return (vocab + kStatChunk - 1) / kStatChunk; }
 int launch_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *first, const int32_t *parents,
                      const int32_t *prefix, const float *rope_cos, const float *rope_sin, int half, int context,
                      int32_t *rows, int32_t *positions, uint32_t *mask, float *cos, float *sin) {
-    tree_plan_kernel<<<n + 1, kPlanThreads, 0, ctx->stream>>>(n, M, max_nodes, (max_nodes + 31) / 32, first, parents,
-                                                              prefix, rope_cos, rope_sin, half, context, rows,
-                                                              positions, mask, cos, sin);
+    const bool wide =
+        half % 4 == 0 &&
+        (((uintptr_t)rope_cos | (uintptr_t)rope_sin | (uintptr_t)cos | (uintptr_t)sin) & 15) == 0;
+    // a round of the rotation rows a workgroup
+    const int64_t items = (int64_t)max_nodes * (wide ? half / 4 : half);
+    const int pieces = (int)(items <= 2 * kPlanThreads ? 1 : items >= 8 * 2 * kPlanThreads ? 8 : items / (2 * kPlanThreads));
+    tree_plan_kernel<<<dim3((unsigned)n + 1, (unsigned)pieces), kPlanThreads, 0, ctx->stream>>>(
+        n, M, max_nodes, (max_nodes + 31) / 32, first, parents, prefix, rope_cos, rope_sin, half, context, wide, rows,
+        positions, mask, cos, sin);
     return check_launch("plan of drafted trees");
 }
 
-// The walks' shares, target and draft chunk sums, chunk maxima, and the greedy picks.
+// The walks' shares, target and draft chunk sums and chunk maxima (the greedy
+// walk: the chunks' best tokens and their logits).
 size_t tree_verify_workspace(int n, int M, int vocab) {
     const size_t cells = (size_t)2 * M * stat_chunks(vocab);
-    return up256((size_t)n * sizeof(Share)) + up256(cells * 8) + up256(cells * 4) + up256((size_t)M * 4);
+    return up256((size_t)n * sizeof(Share)) + up256(cells * 8) + up256(cells * 4);
 }
 
 int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
@@ -759,7 +892,7 @@ int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, 
     Share *share = (Share *)workspace;
     double *sums = (double *)(workspace + up256((size_t)n * sizeof(Share)));
     float *tops = (float *)((uint8_t *)sums + up256(cells * 8));
-    int32_t *picks = (int32_t *)((uint8_t *)tops + up256(cells * 4));
+    int32_t *picks = (int32_t *)sums;
     const bool greedy = temperature == 0.0f;
     const int parts = (vocab + kPart - 1) / kPart, each = kWalkGroups / n;
     const int groups = greedy || M == 0 ? 1 : parts < each ? parts : each > 0 ? each : 1;
@@ -787,7 +920,9 @@ int launch_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, 
                      next};
     if (M == 0) {  // empty trees only
     } else if (greedy) {
-        if (int rc = launch_argmax(ctx, logits, ldl, M, vocab, picks, nullptr, 0, nullptr, nullptr))
+        verify_best_kernel<<<dim3((unsigned)chunks, (unsigned)M), kStatThreads, 0, ctx->stream>>>(logits, ldl, vocab, tops,
+                                                                                                  picks);
+        if (int rc = check_launch("best tokens of drafted trees"))
             return rc;
     } else {
         verify_stats_kernel<<<dim3((unsigned)chunks, (unsigned)M, draft ? 2u : 1u), kStatThreads, 0, ctx->stream>>>(

@@ -673,8 +673,7 @@ int gx_qwen_attention_tree(gx_ctx *ctx, const uint16_t *qh, int n, int M, int ma
  * -inf, takes no child and gives next -1 (greedy: gx_argmax's rule); where the
  * draft's row is such a one the walk takes no child and draws from p.  Computed
  * in float64.  uniforms may be NULL at temperature 0 only.  workspace as
- * above; at temperature 0 the call also uses gx_argmax's scratch, with its
- * rule.  vocab at most 2^20. */
+ * above.  vocab at most 2^20. */
 int gx_tree_verify_workspace_bytes(int n, int M, int vocab, size_t *bytes);
 int gx_tree_verify(gx_ctx *ctx, const float *logits, int ldl, int n, int M, int max_nodes, int vocab,
                    const int32_t *first, const int32_t *parents, const int32_t *tokens, const float *draft_logits,
