@@ -183,42 +183,45 @@ constexpr int kWalkThreads = 256;
 constexpr int kPart = 2048;       // tokens a part of a running sum, eight a thread
 constexpr int kParts = kVocabMax / kPart;
 constexpr int kCells = 1536;      // chunks' statistics a walk stages at a time
-constexpr int kWalkGroups = 512;  // workgroups of a walk, over all its trees
+constexpr int kWalkGroups = 640;  // workgroups of a walk, over all its trees (three fit a CU)
 
-// e^((x - top) / T) as 2^(y / 32), y = (x - top) 32 / (T ln 2): n = y rounded
-// by adding 1.5 * 2^52, whose low bits are then n's; 2^((y - n) / 32) by its
-// Taylor series to the fifth power (3e-15 off), times 2^(n mod 32 / 32) from a
-// table in LDS (32 entries, each on banks of its own), n div 32 added to its
-// exponent: twelve float64 operations, none of the slow kinds (rounding, ldexp
-// and int conversions).  y is held at -1023 * 32, where exponent and table
-// give the bits of zero: a chance below 2^-1022 is none, and so is that of
-// -inf.  NaN and +inf are not told apart here: their row's sum is NaN.
+// e^((x - top) / T) as 2^(y / 64), y = (x - top) 64 / (T ln 2): n = y rounded
+// by adding 1.5 * 2^52, whose low bits are then n's; 2^((y - n) / 64) by its
+// Taylor series to the fourth power (4e-14 off), times 2^(n mod 64 / 64) from a
+// table in LDS whose high words lack their index times 2^14, so that n times
+// 2^14 added puts n div 64 into the exponent: eleven float64 operations, none
+// of the slow kinds (rounding, ldexp and int conversions), and three others.
+// y is held at -1023 * 64, where that gives the bits of zero: a chance below
+// 2^-1022 is none, and so is that of -inf.  NaN and +inf are not told apart
+// here: their row's sum is NaN.
 struct Exp64 {
     double A, top, least;
     const double *table;
     __device__ Exp64(const double *lds, double inv, double t)
-        : A(inv * 0x1.71547652b82fep+5), top(t == -INFINITY ? 0.0 : t), table(lds) {
-        least = -32736.0 / A;
+        : A(inv * 0x1.71547652b82fep+6), top(t == -INFINITY ? 0.0 : t), table(lds) {
+        least = -65472.0 / A;
     }
     __device__ __forceinline__ double operator()(float x) const {
         const double d = fmax((double)x - top, least);
         const double z = __builtin_fma(d, A, 0x1.8p+52);
         const double f = __builtin_fma(d, A, 0x1.8p+52 - z);
-        double p = 0x1.5d87fe78a6730p-35;  // ln2^5 / 120 / 32^5, and so down
-        p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-27);
-        p = __builtin_fma(p, f, 0x1.c6b08d704a0bfp-20);
-        p = __builtin_fma(p, f, 0x1.ebfbdff82c58ep-13);
-        p = __builtin_fma(p, f, 0x1.62e42fefa39efp-6);
+        double p = 0x1.3b2ab6fba4e77p-31;  // ln2^4 / 24 / 64^4, and so down
+        p = __builtin_fma(p, f, 0x1.c6b08d704a0bfp-23);
+        p = __builtin_fma(p, f, 0x1.ebfbdff82c58ep-15);
+        p = __builtin_fma(p, f, 0x1.62e42fefa39efp-7);
         const uint32_t n = (uint32_t)__double2loint(z);
-        const double t = table[n & 31];
-        const double s = __hiloint2double((int)((uint32_t)__double2hiint(t) + ((n & ~31u) << 15)), __double2loint(t));
+        const double t = table[n & 63];
+        const double s = __hiloint2double((int)((n << 14) + (uint32_t)__double2hiint(t)), __double2loint(t));
         return __builtin_fma(s * f, p, s);
     }
 };
 
+constexpr int kTable = 64;
 __device__ __forceinline__ void exp64_table(double *lds) {
-    if (threadIdx.x < 32)
-        lds[threadIdx.x] = kExp2Sixtyfourths[2 * threadIdx.x];
+    if (threadIdx.x < kTable) {
+        const double t = kExp2Sixtyfourths[threadIdx.x];
+        lds[threadIdx.x] = __hiloint2double((int)((uint32_t)__double2hiint(t) - (threadIdx.x << 14)), __double2loint(t));
+    }
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
     constexpr int kMine = kStatChunk / kStatThreads;
     __shared__ float wt[kStatThreads / 64];
     __shared__ double wsum[kStatThreads / 64];
-    __shared__ double table[32];
+    __shared__ double table[kTable];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.y, c0 = blockIdx.x * kStatChunk;
     const float *x = blockIdx.z ? draft + (size_t)row * ldd : logits + (size_t)row * ldl;
@@ -298,9 +301,12 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
             v[k] = i < vocab ? w : -INFINITY;
         }
     }
+    // (a maximum that a NaN goes through: one instruction for two tokens tells of
+    // NaN and +inf too)
 #pragma unroll
     for (int k = 0; k < kMine; k++)
-        top = fmaxf(top, v[k]);
+        top = __builtin_elementwise_maximum(top, v[k]);
+    const bool bad = __ballot(!(top < INFINITY)) != 0;
     top = wave_max(top);
     if (lane == 0)
         wt[wave] = top;
@@ -309,12 +315,9 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
         top = fmaxf(top, wt[w]);
     const Exp64 e(table, blockIdx.z ? itd : it, top);
     double sum = 0.0;
-    bool bad = false;
 #pragma unroll
-    for (int k = 0; k < kMine; k++) {
+    for (int k = 0; k < kMine; k++)
         sum += e(v[k]);
-        bad |= !(v[k] < INFINITY);
-    }
     if (bad)
         sum = NAN;
     sum = wave_sum64(sum);
@@ -481,6 +484,22 @@ struct Helper {
     }
 };
 
+// The least of the workgroup's `hit`s, or where there is none the largest of
+// its `some`s (in every thread).
+__device__ __forceinline__ int first_of(int hit, int some, int *wmin) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // (one minimum for both: hits as they are, the others behind them, largest first)
+    const int key = wave_min_i32(hit != 0x7fffffff ? hit : 0x7ffffffe - some);
+    __syncthreads();
+    if (lane == 0)
+        wmin[wave] = key;
+    __syncthreads();
+    int least = wmin[0];
+    for (int w = 1; w < kWalkThreads / 64; w++)
+        least = min(least, wmin[w]);
+    return least <= kVocabMax ? least : 0x7ffffffe - least;
+}
+
 constexpr int kPolls = 400;  // looks for a walk that has begun, before a helper ends
 
 // grid (groups, n): a tree's first workgroup walks, the others help.
@@ -488,12 +507,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     __shared__ int par[kTreeNodes], tok[kTreeNodes], gone[kTreeNodes];
     __shared__ double px[kTreeNodes], qx[kTreeNodes];                        // a node's token by its parent's rows
     __shared__ double top[kTreeNodes], sum[kTreeNodes], dtop[kTreeNodes], dsum[kTreeNodes];  // a node's own rows
-    __shared__ double run[kParts], own[kParts], table[32], wsum[kWalkThreads / 64];
-    __shared__ double csum[kCells];
-    __shared__ float ctop[kCells];
+    // (the chunks' statistics are read before the first running sum is written:
+    // with them apart two workgroups fit a CU, and not three)
+    __shared__ __align__(16) uint8_t both[kCells * 12];
+    static_assert(kCells * 12 >= kParts * 16, "the running sums fit");
+    double *const csum = (double *)both, *const run = (double *)both, *const own = run + kParts;
+    float *const ctop = (float *)(both + kCells * 8);
+    __shared__ double table[kTable], wsum[kWalkThreads / 64];
+    __shared__ int wmin[kWalkThreads / 64];
     __shared__ float un[kTreeNodes];
     __shared__ unsigned long long got, what[8];
-    __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y;
     const int f0 = min(max(a.first[b], 0), a.M), T = min(min(max(a.first[b + 1], f0), a.M) - f0, a.max_nodes);
     const int parts = (a.vocab + kPart - 1) / kPart;
@@ -617,10 +640,11 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 mx = fmaxf(mx, ctop[i * a.chunks + c]);
             const Exp64 e(table, z ? a.itd : a.it, mx);
             double s = 0.0;
+#pragma unroll 4
             for (int c = 0; c < a.chunks; c++) {
                 const double cs = csum[i * a.chunks + c];
-                if (cs != 0.0)
-                    s += cs - cs == 0.0 ? cs * e(ctop[i * a.chunks + c]) : cs;
+                const double w = cs * e(ctop[i * a.chunks + c]);
+                s += cs == 0.0 ? 0.0 : cs - cs == 0.0 ? w : cs;
             }
             (z ? dtop : top)[node] = mx;
             (z ? dsum : sum)[node] = s;
@@ -725,9 +749,9 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                 if (!help.one(got))
                     break;
             }
-            if (tid == 0)
-                while (share_load(&sh.fin) < (unsigned)parts)
-                    __builtin_amdgcn_s_sleep(1);
+            if (wave == 0)  // every wavefront's own wait would be one more at the same word
+                while (share_load(&sh.fin) < (unsigned)parts) {
+                }
             share_order();
             __syncthreads();
             // the parts' running sum: two of them a thread, over the wavefronts
@@ -772,26 +796,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         const double aim = (double)un[0] * all;
         // the first part that adds to the running sum and at whose end it is past
         // the aim, or the last that adds to it
-        if (tid == 0)
-            found = 0x7fffffff;
-        __syncthreads();
-        int k = -1;
+        int k = 0x7fffffff, some = -1;
         for (int i = tid; i < parts; i += kWalkThreads)
             if (own[i] > 0.0) {
-                k = i;
+                some = i;
                 if (run[i] > aim)
-                    atomicMin(&found, i);
+                    k = min(k, i);
             }
-        __syncthreads();
-        if (found == 0x7fffffff) {
-            __syncthreads();
-            if (tid == 0)
-                found = -1;
-            __syncthreads();
-            atomicMax(&found, k);
-            __syncthreads();
-        }
-        k = found;
+        k = first_of(k, some, wmin);
         const double s = k > 0 ? run[k - 1] : 0.0;
         // the part's running sum: eight tokens in a row a thread
         constexpr int kEach = kPart / kWalkThreads;
@@ -817,16 +829,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             if (lane >= d)
                 up += o;
         }
-        __syncthreads();
-        if (tid == 0)
-            found = 0x7fffffff;
         if (lane == 63)
             wsum[wave] = up;
         __syncthreads();
         double at = s + (up - mine);
         for (int i = 0; i < wave; i++)
             at += wsum[i];
-        int hit = 0x7fffffff, some = -1;
+        int hit = 0x7fffffff;
+        some = -1;  // (where rounding passed the aim by: the last token with a chance)
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
             at += w[i];
@@ -836,19 +846,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
                     hit = x0 + i;
             }
         }
-        if (hit != 0x7fffffff)
-            atomicMin(&found, hit);
-        __syncthreads();
-        token = found;
-        if (token == 0x7fffffff) {  // the running sum's rounding passed the aim by: the last token with a chance
-            __syncthreads();
-            if (tid == 0)
-                found = -1;
-            __syncthreads();
-            atomicMax(&found, some);
-            __syncthreads();
-            token = found;
-        }
+        token = first_of(hit, some, wmin);
     }
     if (tid == 0) {
         a.counts[b] = kept;
