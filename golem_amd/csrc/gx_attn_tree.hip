@@ -376,8 +376,8 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
     const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head >= x.heads)
         return;
-    int b = -1;  // the tree: the last whose first token is not past this one
-    for (int i = 0; i < x.n; i += 64)
+    int b = x.n == 1 ? 0 : -1;  // the tree: the last whose first token is not past this one
+    for (int i = 0; x.n > 1 && i < x.n; i += 64)
         b += __popcll(__ballot(i + lane < x.n && x.first[min(i + lane, x.n - 1)] <= tok));
     const Tree t(x, max(b, 0));
     if (b < 0 || tok < t.f0 || tok >= t.f0 + t.T)

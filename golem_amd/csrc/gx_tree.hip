@@ -237,14 +237,16 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // that finds none walking after a while ends, and so do all when the walk does.
 struct Share {
     unsigned long long claim;  // the sum's number in the high half, the next part in the low
-    alignas(128) unsigned fin; // parts that are summed
-    // the open sum (eight words: one load of a wavefront's lanes): the row and
-    // the tokens turned down, then the row's largest logit and the factor of its
-    // exponentials in what is left, and the draft's
+    // the open sum (six words: one load and one store of a wavefront's lanes): the
+    // row and the tokens turned down, then the row's largest logit and the factor
+    // of its exponentials in what is left, and the draft's
     alignas(128) unsigned long long what[8];
-    alignas(128) double part[kParts];
+    // the parts' sums, kNone until they are there; odd and even sums apart, so that
+    // the next one's can be cleared while this one's are on their way
+    alignas(128) unsigned long long part[2][kParts];
     int gone[kTreeNodes];
 };
+constexpr unsigned long long kNone = ~0ull;  // (the bits of no sum: a logit's NaN has low bits of zero)
 // claims before the first sum and after the last (a late asker's count stays in the low half)
 constexpr unsigned long long kWalking = 1, kWalked = 0xFFFFFFFF00000000ull;
 
@@ -475,11 +477,8 @@ struct Helper {
                         turned,
                         a.vocab};
         const double s = part_sum(left, k, wsum);
-        if (tid == 0) {
-            share_store(&sh.part[k], s);
-            share_order();
-            share_add(&sh.fin, 1u);
-        }
+        if (tid == 0)
+            share_store(&sh.part[old >> 32 & 1][k], (unsigned long long)__double_as_longlong(s));
         return true;
     }
 };
@@ -565,8 +564,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         return;
     }
-    if (tid == 0 && !a.picks)
-        share_store(&sh.claim, kWalking);
+    // the parts' sums of a parity, none of them there
+    auto clear = [&](int parity) __attribute__((always_inline)) {
+        for (int i = tid; i < parts; i += kWalkThreads)
+            share_store(&sh.part[parity][i], kNone);
+    };
+    if (!a.picks) {
+        if (tid == 0)
+            share_store(&sh.claim, kWalking);
+        clear(1);
+    }
     exp64_table(table);
     for (int i = tid; i < T; i += kWalkThreads) {
         par[i] = a.parents[f0 + i];
@@ -726,38 +733,47 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         const bool ending = m >= T;
         if (!summed) {
             // the sum of what is left of v's row, handed out
-            if (tid == 0) {
-                const int listed = a.draft ? 0 : turned;
-                const double words[] = {1.0 / sum[v], off()};
-                share_store(&sh.what[0], (unsigned long long)(f0 + v));
-                share_store(&sh.what[1], (unsigned long long)listed);
-                share_store(&sh.what[2], (unsigned long long)__double_as_longlong(top[v]));
-                share_store(&sh.what[3], (unsigned long long)__double_as_longlong(words[0]));
-                share_store(&sh.what[4], (unsigned long long)__double_as_longlong(a.draft ? dtop[v] : 0.0));
-                share_store(&sh.what[5], (unsigned long long)__double_as_longlong(words[1]));
-                for (int i = 0; i < listed; i++)
-                    share_store(&sh.gone[i], gone[i]);
-                share_store(&sh.fin, 0u);
-                share_order();
-                share_store(&sh.claim, (unsigned long long)++sums << 32);
+            const int listed = a.draft ? 0 : turned;
+            sums++;
+            if (tid < 6) {
+                const double words[6] = {0.0, 0.0, top[v], 1.0 / sum[v], a.draft ? dtop[v] : 0.0, off()};
+                unsigned long long mine = tid == 0 ? (unsigned long long)(f0 + v) : (unsigned long long)listed;
+#pragma unroll
+                for (int i = 2; i < 6; i++)
+                    mine = tid == i ? (unsigned long long)__double_as_longlong(words[i]) : mine;
+                share_store(&sh.what[tid], mine);
             }
-            for (;;) {
-                __syncthreads();
-                if (tid == 0)
-                    got = share_add(&sh.claim, 1ull);
-                __syncthreads();
-                if (!help.one(got))
-                    break;
-            }
-            if (wave == 0)  // every wavefront's own wait would be one more at the same word
-                while (share_load(&sh.fin) < (unsigned)parts) {
-                }
+            for (int i = tid; i < listed; i += kWalkThreads)
+                share_store(&sh.gone[i], gone[i]);
             share_order();
             __syncthreads();
-            // the parts' running sum: two of them a thread, over the wavefronts
+            if (tid == 0) {
+                share_store(&sh.claim, (unsigned long long)sums << 32);
+                got = share_add(&sh.claim, 1ull);
+            }
+            clear((sums + 1) & 1);
+            __syncthreads();
+            help.one(got);
+            // the parts' sums, two of them a thread, as they come; where there are more
+            // parts than workgroups, or they are long in coming, another part itself
             static_assert(kParts == 2 * kWalkThreads, "two parts a thread");
-            const double one = 2 * tid < parts ? share_load(&sh.part[2 * tid]) : 0.0;
-            const double two = 2 * tid + 1 < parts ? share_load(&sh.part[2 * tid + 1]) : 0.0;
+            const unsigned long long *from = sh.part[sums & 1] + 2 * tid;
+            unsigned long long w1 = 2 * tid < parts ? kNone : 0ull, w2 = 2 * tid + 1 < parts ? kNone : 0ull;
+            for (int looks = 1;; looks++) {
+                if (w1 == kNone)
+                    w1 = share_load(from);
+                if (w2 == kNone)
+                    w2 = share_load(from + 1);
+                if (!__syncthreads_or(w1 == kNone || w2 == kNone))
+                    break;
+                if (parts > a.groups || looks % 8 == 0) {
+                    if (tid == 0)
+                        got = share_add(&sh.claim, 1ull);
+                    __syncthreads();
+                    help.one(got);
+                }
+            }
+            const double one = __longlong_as_double((long long)w1), two = __longlong_as_double((long long)w2);
             double up = one + two;
             for (int d = 1; d < 64; d <<= 1) {
                 const double o = __shfl_up(up, d);
