@@ -438,7 +438,9 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
     for (int i = 0; i < 4; i++)
         y[i] = any ? o[i] / l : 0.0f;
     const size_t at = (size_t)tok * width + head * HD + e;
-    if (out)
+    if (out && ((uintptr_t)out & 15) == 0)
+        *(v4f *)(out + at) = y;
+    else if (out)
         for (int i = 0; i < 4; i++)
             out[at + i] = y[i];
     if (q8) {
@@ -446,8 +448,11 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
         float stored;
         int32_t sm;
         const uint32_t packed = q8_0_quad(v, &stored, &sm);
-        for (int i = 0; i < 4; i++)
-            q8[at + i] = (int8_t)(packed >> (8 * i));
+        if (((uintptr_t)q8 & 3) == 0)
+            *(uint32_t *)(q8 + at) = packed;
+        else
+            for (int i = 0; i < 4; i++)
+                q8[at + i] = (int8_t)(packed >> (8 * i));
         if ((lane & 7) == 0) {
             scales[at >> 5] = stored;
             qsum[at >> 5] = sm;

@@ -165,7 +165,7 @@ class QwenModel:
         self.graph = None
         self.slot_graphs = {}
         self.drafts = 0  # tokens the draft buffers hold (set_drafts)
-        self.tree_ws = None
+        self.tree_ws, self.tree_ws_kept = None, []
         n = capi.size_out("gx_qwen_attention_workspace_bytes", M, cfg.heads, cfg.max_context - 1)
         self.attn_ws = torch.empty((n + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
         self._vp, self._call = vp, call
@@ -592,6 +592,7 @@ class QwenModel:
     def _tree_workspace(self, name, *size):
         n = (capi.size_out(name, *size) + 255) // 256 * 256
         if self.tree_ws is None or self.tree_ws.numel() < n:
+            self.tree_ws_kept.append(self.tree_ws)  # a captured pass may hold its address
             self.tree_ws = torch.empty(n, dtype=torch.uint8, device="cuda")
         return self._vp(self.tree_ws), self.tree_ws.numel()
 

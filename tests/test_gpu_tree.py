@@ -87,6 +87,13 @@ def test_plan(dev, sizes, fanout, max_nodes, pad):
     run_plan(dev, sizes, parents, prefix, 600, 32, max_nodes, sum(sizes) + pad)
 
 
+@pytest.mark.parametrize("half", [1, 5, 12, 64, 128])
+def test_plan_rotation_rows(dev, half):
+    """Head widths off the 16-byte pieces, and rows past one workgroup's."""
+    sizes = [70, 3, 33]
+    run_plan(dev, sizes, random_parents(synth.rng(2), sizes, 3), np.array([9, 0, 4]), 100, half, 70, 110)
+
+
 def test_plan_leaves_out_what_has_no_place(dev):
     # a later parent, itself, below -1, and everything below those; a second
     # root; positions past the context; a negative prefix; more nodes than max_nodes
@@ -737,6 +744,29 @@ def test_a_tree_gives_each_path_its_own_pass(dev):
     m.free()
 
 
+def test_a_tree_in_the_products_epilogue(dev):
+    """More than sixteen drafted tokens: the Q|K|V product stores the drafts'
+    heads itself.  Each node's hidden state is that of a smaller pass of its
+    path alone."""
+    g = synth.rng(64)
+    prompt = [int(t) for t in g.integers(0, CFG.vocab, 10)]
+    parents = [-1] + [int(g.integers(max(0, i - 6), i)) for i in range(1, 27)]
+    tokens = [int(t) for t in g.integers(0, CFG.vocab, 27)]
+    m = _model(dev)
+    m.set_drafts(27)
+    m.forward(prompt, 0)
+    got = m.forward_tree([tokens], [parents], [len(prompt)]).cpu().numpy().copy()
+    for i in range(27):
+        path, x = [], i
+        while x >= 0:
+            path.insert(0, tokens[x])
+            x = parents[x]
+        assert len(path) <= 16
+        h = m.forward_tree([path], [[-1] + list(range(len(path) - 1))], [len(prompt)])[-1].cpu().numpy()
+        _close(got[i], h)
+    m.free()
+
+
 def _oracle_draft(ids, sequence, width):
     """Three tokens along the sequence with a wrong one in some places, and `width` - 1 wrong siblings of each."""
     tokens, parents, up = [], [], 0
@@ -889,6 +919,37 @@ def test_captured_pass_equals_eager(dev):
         for a, b in zip(*results):
             assert t.equal(a, b)
     m.free()
+
+
+def test_two_verifications_at_once(dev):
+    """Walks of two contexts on two streams together, more workgroups than the
+    GPU holds: neither waits for the other's."""
+    t = torch
+    ctxs, cases, held = [], [], []
+    for k in range(2):
+        sizes = [6] * 8
+        parents, tokens, logits, draft, u = make_verify(90 + k, sizes, 2, 151936, True)
+        args = (sizes, parents, tokens, logits, draft, 1.0, 1.0, u, 6)
+        cases.append((args, verify_reference(*args)))
+        s = t.cuda.Stream()
+        ctxs.append((capi.Context(0, stream=s.cuda_stream), s))
+        M = sum(sizes)
+        size = capi.size_out("gx_tree_verify_workspace_bytes", 8, M, 151936)
+        held.append([dev.put(x) for x in (logits, draft, offsets(sizes), parents, tokens, u)]
+                    + [dev.empty((8, 6), np.int32), dev.empty((8,), np.int32), dev.empty((8,), np.int32),
+                       dev.empty((size,), np.uint8)])
+    t.cuda.synchronize()
+    for _ in range(20):
+        for (ctx, s), x in zip(ctxs, held):
+            lg, dr, first, par, tok, u, path, counts, nxt, ws = x
+            capi.call("gx_tree_verify", ctx.ptr, vp(lg), 151936, 8, 48, 6, 151936, vp(first), vp(par), vp(tok), vp(dr),
+                      151936, 1.0, 1.0, vp(u), vp(path), vp(counts), vp(nxt), vp(ws), ws.numel())
+    t.cuda.synchronize()
+    for (_, want), x in zip(cases, held):
+        for got, w in zip(x[6:9], want):
+            np.testing.assert_array_equal(got.cpu().numpy(), w)
+    for ctx, _ in ctxs:
+        ctx.close()
 
 
 def test_two_contexts_on_their_own_streams(dev):
