@@ -1101,7 +1101,8 @@ int gx_qwen_tree_plan(gx_ctx *ctx, int n, int M, int max_nodes, const int32_t *f
                       int32_t *rows, int32_t *positions, uint32_t *mask, float *cos, float *sin) {
     if (int rc = check_trees(n, M, max_nodes))
         return rc;
-    GX_CHECK(half > 0 && context > 0, "gx: rotation tables of %d rows of %d", context, half);
+    GX_CHECK(half > 0 && half <= 512 && context > 0, "gx: rotation tables of %d rows of %d (at most 512)", context,
+             half);
     GX_CHECK(first && parents && prefix && rope_cos && rope_sin && rows && positions && mask && cos && sin,
              "gx: missing argument");
     if (int rc = use(ctx))
@@ -1214,6 +1215,7 @@ static int check_layers(int layers, int kv_heads, int head_dim, int context, uin
     GX_CHECK(layers > 0 && kv_heads > 0 && kv_heads <= 65535 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= 1024,
              "gx: caches of %d layers, %d key-value heads of %d", layers, kv_heads, head_dim);
     GX_CHECK(context > 0 && context % 8 == 0, "gx: a cache of %d positions (a multiple of 8)", context);
+    GX_CHECK((int64_t)context * head_dim <= INT32_MAX, "gx: a head of %d positions is too long", context);
     GX_CHECK(kcaches && vcaches, "gx: missing argument");
     for (int l = 0; l < layers; l++)
         GX_CHECK(kcaches[l] && vcaches[l] && (((uintptr_t)kcaches[l] | (uintptr_t)vcaches[l]) & 15) == 0,

@@ -611,7 +611,7 @@ int gx_argmax_slots_step(gx_ctx *ctx, const float *x, int ldx, int M, int n, int
  * = prefix[b] + depth, mask[m] (ceil(max_nodes/32) words) with bit j % 32 of
  * word j / 32 set where node j is node m's ancestor or itself, and cos[m] /
  * sin[m] = row positions[m] of rope_cos / rope_sin ([context][half] floats,
- * half = head_dim / 2).  A node whose parent is neither an earlier node nor -1,
+ * half = head_dim / 2, at most 512).  A node whose parent is neither an earlier node nor -1,
  * every node below such a one, a node past `context`, and a token of no tree
  * have no place: rows and positions -1, mask, cos and sin zero (gx_qwen_qk_rope
  * then stores nothing and makes their query NaN).  All device pointers. */
@@ -695,7 +695,8 @@ int gx_qwen_cache_commit(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint
 
 /* Conversation src's positions 0 .. len - 1 into conversations dsts[0..n)
  * (host ints, all different and not src), all layers; the rest of those
- * conversations' caches stays.  kcaches, vcaches: host arrays as above. */
+ * conversations' caches stays.  kcaches, vcaches: host arrays as above.  (Here
+ * and in the calls above a head's context * head_dim is below 2^31.) */
 int gx_qwen_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16_t *const *vcaches, int nslots,
                        int kv_heads, int head_dim, int context, int src, const int32_t *dsts, int n, int len);
 

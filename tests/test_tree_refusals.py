@@ -27,7 +27,8 @@ PLAN = dict(ctx=None, n=1, M=4, max_nodes=4, first=A, parents=A, prefix=A, cos=A
 @pytest.mark.parametrize("changes,message", [
     ({}, "no context"), ({"n": -1}, "trees"), ({"n": 1025}, "at most 1024"), ({"M": -1}, "tokens"),
     ({"M": 65536}, "at most 65535"), ({"max_nodes": 0}, "trees of 0 nodes"), ({"max_nodes": 513}, "1 to 512"),
-    ({"half": 0}, "rotation tables"), ({"context": 0}, "rotation tables"), ({"parents": None}, "missing"),
+    ({"half": 0}, "rotation tables"),
+    ({"half": 513}, "at most 512"), ({"context": 0}, "rotation tables"), ({"parents": None}, "missing"),
     ({"os": None}, "missing"),
 ])
 def test_plan(changes, message):
@@ -91,7 +92,7 @@ COMMIT = dict(ctx=None, layers=2, kc=_layers(A, A), vc=_layers(A, A), kd=_layers
     ({}, "no context"), ({"layers": 0}, "0 layers"), ({"kc": _layers(A, None)}, "layer 1"),
     ({"vc": _layers(A + 2, A)}, "layer 0"), ({"kd": _layers(A, A + 4)}, "layer 1"), ({"vd": _layers(None, A)}, "layer 0"),
     ({"head_dim": 60}, "key-value heads of 60"), ({"context": 12}, "multiple of 8"), ({"draft_context": 2}, "draft buffers"),
-    ({"path": None}, "missing"), ({"slots": A}, "0 slots"), ({"kd": None}, "missing"),
+    ({"context": 1 << 25}, "too long"), ({"path": None}, "missing"), ({"slots": A}, "0 slots"), ({"kd": None}, "missing"),
 ])
 def test_commit(changes, message):
     refused("gx_qwen_cache_commit", _change(COMMIT, changes), message)
@@ -109,7 +110,7 @@ FORK = dict(ctx=None, layers=2, kc=_layers(A, A), vc=_layers(A, A), nslots=4, kv
     ({}, "no context"), ({"src": 4}, "slot 4 of 4"), ({"src": -1}, "slot -1"), ({"dsts": _slots(0, 4)}, "slot 4 of 4"),
     ({"dsts": _slots(1, 0)}, "into itself"), ({"dsts": _slots(2, 2)}, "named twice"), ({"n": 4}, "4 forks"),
     ({"n": -1}, "-1 forks"), ({"len": 65}, "65 positions"), ({"len": -1}, "-1 positions"), ({"kc": None}, "missing"),
-    ({"dsts": None}, "forks among"),
+    ({"dsts": None}, "forks among"), ({"context": 1 << 25}, "too long"),
 ])
 def test_fork(changes, message):
     refused("gx_qwen_cache_fork", _change(FORK, changes), message)
