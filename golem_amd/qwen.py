@@ -166,6 +166,7 @@ class QwenModel:
         self.slot_graphs = {}
         self.drafts = 0  # tokens the draft buffers hold (set_drafts)
         self.tree_ws, self.tree_ws_kept = None, []
+        self.tree_states = False  # the hidden states are forward_tree's
         n = capi.size_out("gx_qwen_attention_workspace_bytes", M, cfg.heads, cfg.max_context - 1)
         self.attn_ws = torch.empty((n + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
         self._vp, self._call = vp, call
@@ -290,6 +291,7 @@ class QwenModel:
         (forward), whose caches the attention then reads as a lone
         conversation's."""
         cfg, vp, call, ctx = self.cfg, self._vp, self._call, self.ctx.ptr
+        self.tree_states = False
         call("gx_weight_rows", ctx, self.embd.ptr, 0, vp(self.tokens), M, vp(self.xs))
         if M == 1:
             return self._blocks_one(max_pos)
@@ -452,6 +454,7 @@ class QwenModel:
         top = max(self._slot_pos)
         if top >= self.slot_context:
             raise ValueError(f"qwen: position {top} is past a slot's {self.slot_context}")
+        self.tree_states = False
         if graph:
             self.capture_slots(n)
             self.slot_graphs[n].replay()
@@ -559,6 +562,7 @@ class QwenModel:
         also recorded as the history's entry `pos`."""
         if pos >= self.cfg.max_context:
             raise ValueError(f"qwen: position {pos} is past the context {self.cfg.max_context}")
+        self.tree_states = False
         self.tokens[:1].copy_(tok)
         self.history[pos:pos + 1].copy_(tok)
         self.pos_dev.fill_(pos)
@@ -636,8 +640,8 @@ class QwenModel:
         self.tree = {"n": n, "M": M, "nodes": nodes, "first": dev(first), "parents": dev(flat(parents)),
                      "prefix": dev(prefixes), "slots": dev(slots), "max_prefix": int(max(prefixes)),
                      "mask": torch.empty((M, (nodes + 31) // 32), dtype=torch.int32, device="cuda"),
-                     "path": torch.empty((n, nodes), dtype=torch.int32, device="cuda"),
-                     "counts": torch.empty((n,), dtype=torch.int32, device="cuda"),
+                     "path": torch.full((n, nodes), -1, dtype=torch.int32, device="cuda"),
+                     "counts": torch.zeros((n,), dtype=torch.int32, device="cuda"),
                      "next": torch.empty((n,), dtype=torch.int32, device="cuda")}
         self._tree_blocks(self.tree)
         return self.hidden[:M]
@@ -647,8 +651,9 @@ class QwenModel:
         device state alone (so that it can be captured, the workspace being
         there)."""
         cfg, vp, call, ctx = self.cfg, self._vp, self._call, self.ctx.ptr
-        n, M, nodes, qd = t["n"], t["M"], t["nodes"], self.qd
+        n, M, nodes = t["n"], t["M"], t["nodes"]
         eps = np.float32(cfg.eps)
+        self.tree_states = True
         call("gx_qwen_tree_plan", ctx, n, M, nodes, vp(t["first"]), vp(t["parents"]), vp(t["prefix"]),
              vp(self.rope_cos), vp(self.rope_sin), cfg.head_dim // 2, self.slot_context, vp(self.draft_rows),
              vp(self.positions), vp(t["mask"]), vp(self.draft_cos), vp(self.draft_sin))
@@ -683,10 +688,13 @@ class QwenModel:
         (device float32 [M], in [0, 1); default: torch's generator) decides,
         the drafts being given tokens or, with draft_logits (device [M][vocab],
         the draft model's logits after each node), drawn from their softmax at
-        draft_temperature (default: temperature).  Returns device tensors:
+        draft_temperature (default: temperature).  No other pass may have run
+        since.  Returns device tensors:
         path [trees][nodes] (-1 behind), counts [trees], next [trees]."""
         t, vp, V = self._a_tree(), self._vp, self.cfg.vocab
         M = t["M"]
+        if not self.tree_states:
+            raise ValueError("qwen: another pass has replaced the drafted tokens' states")
         if uniforms is None and temperature > 0:
             uniforms = torch.rand((M,), device="cuda")
         for x, shape, what in ((draft_logits, (M, V), "draft logits"), (uniforms, (M,), "random numbers")):
@@ -703,8 +711,9 @@ class QwenModel:
         return t["path"], t["counts"], t["next"]
 
     def commit_tree(self):
-        """The kept paths of the last verify_tree into their conversations'
-        caches: prefixes[b] + counts[b] positions are cached then."""
+        """The kept paths of the last verify_tree (none before it) into their
+        conversations' caches: prefixes[b] + counts[b] positions are cached
+        then."""
         t, vp, cfg = self._a_tree(), self._vp, self.cfg
         layers = [(ctypes.c_void_p * cfg.layers)(*[x.data_ptr() for x in xs])
                   for xs in (self.kc, self.vc, self.kd, self.vd)]
@@ -731,8 +740,8 @@ class QwenModel:
         """`steps` tokens after the prompt, several a pass where drafts are
         kept.  draft(ids) proposes a tree after the ids so far: (tokens,
         parents) of nodes 1, 2, .., parents as node numbers with 0 the last
-        id, or with a third entry, the device draft logits [1 + nodes][vocab]
-        that the tokens were drawn from.  temperature 0: greedy's tokens;
+        id, or with a third entry (or None), the device draft logits
+        [1 + nodes][vocab] that the tokens were drawn from.  temperature 0: greedy's tokens;
         above, random numbers come from `generator` (a torch generator of the
         GPU).  Returns the ids and the number of passes."""
         if not prompt or len(prompt) + steps - 1 > self.slot_context:
@@ -744,7 +753,7 @@ class QwenModel:
             self.forward(ids[at:min(cached, at + self.max_batch)], at)
         while len(ids) < len(prompt) + steps:
             tokens, parents, *logits = draft(list(ids))
-            depth, keep = [0], 1  # nodes within the context, the buffers and the steps asked for
+            depth, keep = [0], 1  # nodes within the context and the buffers
             for p in parents[:self.drafts - 1]:
                 depth.append(depth[p] + 1)
                 if cached + depth[-1] >= self.slot_context:
@@ -753,12 +762,14 @@ class QwenModel:
             tree = [ids[-1]] + [int(x) for x in tokens[:keep - 1]]
             self.forward_tree([tree], [[-1] + list(parents[:keep - 1])], [cached])
             uniforms = None if temperature == 0 else torch.rand((keep,), generator=generator, device="cuda")
-            path, counts, nxt = self.verify_tree(temperature, logits[0][:keep] if logits else None,
+            path, counts, nxt = self.verify_tree(temperature, logits[0][:keep] if logits and logits[0] is not None else None,
                                                  uniforms=uniforms)
             self.commit_tree()
-            count = int(counts[0])
+            count, after = int(counts[0]), int(nxt[0])
+            if after < 0:
+                raise ValueError("qwen: logits that no token can be drawn from")
             kept = path[0, :count].tolist()
-            ids += [tree[i] for i in kept[1:]] + [int(nxt[0])]
+            ids += [tree[i] for i in kept[1:]] + [after]
             cached += count
             passes += 1
         return ids[len(prompt):len(prompt) + steps], passes

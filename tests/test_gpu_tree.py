@@ -872,6 +872,55 @@ def test_model_refusals(dev):
     m.free()
 
 
+def test_passes_in_between(dev):
+    """A pass between forward_tree and verify_tree takes the states away; one
+    after verify_tree does not keep its path from being committed, and before
+    it there is none to commit."""
+    m = _model(dev)
+    m.set_drafts(8)
+    m.forward([4, 5, 6], 0)
+    saved = [x.clone() for x in m.kc + m.vc]
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.commit_tree()
+    for x, y in zip(saved, m.kc + m.vc):
+        assert torch.equal(x, y)
+    m.forward([7], 3)
+    with pytest.raises(ValueError, match="another pass"):
+        m.verify_tree()
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    path, counts, _ = m.verify_tree()
+    want = [x.clone() for x in m.kd]
+    m.forward([8], 20)
+    m.commit_tree()
+    for i in range(int(counts[0])):
+        node = int(path[0, i])
+        for x, y in zip(want, m.kc):
+            assert torch.equal(x[:, :, node], y.reshape(x.shape[0], x.shape[1], -1, 8)[:, :, 3 + i])
+    m.capture_decode()
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.start_decode(torch.tensor([3], dtype=torch.int32, device="cuda"), 5)
+    with pytest.raises(ValueError, match="another pass"):
+        m.verify_tree()
+    m.free()
+
+
+def test_speculation_with_foreign_drafts(dev):
+    """Drafted tokens outside the vocabulary are passed over: their rows are
+    NaN, and nothing of them reaches the others."""
+    m = _model(dev)
+    prompt, steps = [int(t) for t in synth.rng(65).integers(0, CFG.vocab, 6)], 12
+    want = m.greedy(prompt, steps)
+
+    def draft(ids):
+        right = (prompt + want + [1])[len(ids)]
+        return [CFG.vocab + 3, -7, right, right], [0, 1, 0, 1], None
+
+    m.reset()
+    got, passes = m.speculate(prompt, steps, draft)
+    assert got == want and passes <= (steps + 1) // 2
+    m.free()
+
+
 def test_captured_pass_equals_eager(dev):
     """A pass -- forward, verification, commit -- captured once and replayed
     for other tokens and prefixes, with eager work between the replays."""
