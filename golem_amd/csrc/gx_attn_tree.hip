@@ -12,13 +12,18 @@
 // wavefront's halves hold 16 keys each), and with key piece m of a step read
 // from position swap23(m) (bits 2 and 3 exchanged) registers 8t .. 8t + 7 of
 // half h are the keys 16t + 8h .. + 7: the second operand of O^T = V^T P^T as
-// it stands, beside value rows read 16 bytes a lane.  Neither product passes
-// through LDS.
+// it stands, beside value rows read 16 bytes a lane.  Scores and probabilities
+// never leave the registers.
 //
 // A probability enters the second product as two fp16 values, its leading 11
 // bits and the rest (about 22 bits together): rounded to one, the head
 // outputs would be 2e-4 off, which the float output could not hide.  Sums,
 // maxima and outputs are float32.
+//
+// Two kernels and a join of the keys' shares.  Trees of one tile of rows (eight
+// nodes of four query heads a key-value head, say) move bytes more than they
+// compute and take attn_tree_narrow_kernel; where their prefixes are short that
+// is the only launch.  Larger trees take attn_tree_kernel.
 #include <algorithm>
 
 #include "gx_device.hpp"
@@ -34,6 +39,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 32;        // rows a wavefront
 constexpr int kStage = 64;       // keys a step
+constexpr int kNarrow = 32;      // keys a step of the kernel for one tile
 constexpr int kMaxWaves = 8;     // wavefronts a workgroup: a tile of rows each, the keys shared
 constexpr int kMaxSplits = 64;   // shares of the keys, over workgroups
 // Probabilities are held times 2^8, their low parts clear of fp16's
@@ -48,22 +54,26 @@ struct Args {
     const int32_t *prefix;
     const int32_t *slots;
     const uint16_t *kc, *vc, *kd, *vd;
-    int n, M, max_nodes, words, max_prefix, heads, kv_heads, context, draft_context, nslots, S;
+    int n, M, max_nodes, words, max_prefix, heads, kv_heads, context, draft_context, nslots, S, stage;
     float c;       // 1 / sqrt(hd) in the exponent's base 2
     float *po;     // [S][M][heads][hd] unnormalised outputs
     float *pml;    // [S][M][heads][2] maximum (base 2) and sum
+    float *out;    // the results, each optional
+    int8_t *q8;
+    float *scales;
+    int32_t *qsum;
 };
 
 // A tree's tokens, cached positions and steps, the same for every kernel.
 struct Tree {
     int f0, T, P, a, np, total, per;  // (total and per: steps)
-    __device__ Tree(const Args &x, int b) {
+    __device__ Tree(const Args &x, int b, int stage) {
         f0 = __builtin_amdgcn_readfirstlane(min(max(x.first[b], 0), x.M));
         T = __builtin_amdgcn_readfirstlane(min(min(max(x.first[b + 1], f0), x.M) - f0, x.max_nodes));
         P = __builtin_amdgcn_readfirstlane(min(max(x.prefix[b], 0), min(x.max_prefix, x.context)));
         a = f0 & 7;  // draft rows are read from a multiple of 8
-        np = (P + kStage - 1) / kStage;
-        total = np + (T > 0 ? (a + T + kStage - 1) / kStage : 0);
+        np = (P + stage - 1) / stage;
+        total = np + (T > 0 ? (a + T + stage - 1) / stage : 0);
         per = max(1, (total + x.S - 1) / x.S);
     }
 };
@@ -101,9 +111,35 @@ __device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
 
+// Eight keys' chances (w: which of a step's scores s), their leading 11 bits
+// and the rest, added to l.
+__device__ __forceinline__ void chances(const v16f &s, int w, float c, float base, v8h &ph, v8h &pl, float &l) {
+    uint32_t hb[4], lb[4];
+    float part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[8 * w + 2 * i], c, base));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[8 * w + 2 * i + 1], c, base));
+        part += p + p1;
+        hb[i] = pack_rtz(p, p1);
+        lb[i] = pack_rtz(fma_mix_lo(hb[i], 0xBC00BC00u, p), fma_mix_hi(hb[i], 0xBC00BC00u, p1));
+    }
+    l += part;
+    const v4u hv = {hb[0], hb[1], hb[2], hb[3]}, lv = {lb[0], lb[1], lb[2], lb[3]};
+    ph = __builtin_bit_cast(v8h, hv);
+    pl = __builtin_bit_cast(v8h, lv);
+}
+
 // grid (kv_heads, row groups, trees * S), 64 threads a 32-row tile of the
 // group: key-value heads fastest, so that with eight of them every workgroup
 // of a head is on one XCD and shares its L2.
+//
+// Bound by the matrix instructions: 64 nodes of 32 heads over 8, 128 wide, and
+// 32000 positions take 60 us (48 a step and wavefront at 30 ns each, where a
+// large fp16 product of a library reaches 28), 2.2 TB/s of keys and values; the
+// join 8 us.  A second wavefront a SIMD adds nothing then, nor did scores and
+// products of neighbouring steps side by side (65 us), a longer ring, or an
+// order of the instructions laid down by hand.
 //
 // A step's 64 keys and values come into LDS by direct loads, one step ahead of
 // the products, for every tile of the group: the keys as 1 KiB pieces of 64
@@ -117,7 +153,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nw = blockDim.x >> 6, li = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
-    const Tree t(x, b);
+    const Tree t(x, b, kStage);
     const int g = x.heads / x.kv_heads, R = t.T * g, g0 = blockIdx.y * nw * kTile, r0 = g0 + wave * kTile;
     const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
     if (g0 >= R || t0 >= t1)
@@ -169,7 +205,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const uint32_t vlane = HD * 128 + li * 128, vx = h ^ (li & 7);
 
     // the first four wavefronts go first: the others' matrix products then run
-    // beside their exponentials
+    // beside their exponentials (up to 3 us of 60, as the clock allows)
     if (wave < 4)
         __builtin_amdgcn_s_setprio(1);
     v16f o[ET] = {};
@@ -274,23 +310,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
         }
         const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
         v8h ph[4], pl[4];
-        auto chances = [&](int w) __attribute__((always_inline)) {
-            uint32_t hb[4], lb[4];
-            float part = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[w >> 1][8 * (w & 1) + 2 * i], x.c, base));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[w >> 1][8 * (w & 1) + 2 * i + 1], x.c, base));
-                part += p + p1;
-                hb[i] = pack_rtz(p, p1);
-                lb[i] = pack_rtz(fma_mix_lo(hb[i], 0xBC00BC00u, p), fma_mix_hi(hb[i], 0xBC00BC00u, p1));
-            }
-            l += part;
-            const v4u hv = {hb[0], hb[1], hb[2], hb[3]}, lv = {lb[0], lb[1], lb[2], lb[3]};
-            ph[w] = __builtin_bit_cast(v8h, hv);
-            pl[w] = __builtin_bit_cast(v8h, lv);
-        };
-        chances(0);
+        chances(s[0], 0, x.c, base, ph[0], pl[0], l);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
 #pragma unroll
@@ -302,7 +322,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
             if (w < 2)
                 values(w + 2);
             if (w < 3)
-                chances(w + 1);
+                chances(s[(w + 1) >> 1], (w + 1) & 1, x.c, base, ph[w + 1], pl[w + 1], l);
         }
     }
     if (r0 + li >= R)
@@ -326,10 +346,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
 // The elements of a row that a masked value has spoilt (an infinite or NaN
 // value that the mask hides makes 0 * inf in its step), summed again over what
 // the node sees alone: 64 keys at a time, a key a lane, the spoilt elements in
-// turn.  o: the row's outputs, four a lane; spoilt: which of them.
+// turn.  o: four of the row's outputs, from element e on; spoilt: which of them.
 template <int HD>
 __device__ __forceinline__ v4f attn_tree_again(const Args &x, const Tree &t, int b, int tok, int head, float top, v4f o,
-                                            uint32_t spoilt) {
+                                               int e, uint32_t spoilt) {
     const int lane = threadIdx.x & 63, kvh = head / (x.heads / x.kv_heads);
     const int slot = x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0;
     const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
@@ -354,7 +374,7 @@ __device__ __forceinline__ v4f attn_tree_again(const Args &x, const Tree &t, int
             for (int i = 0; i < 4; i++)
                 for (unsigned long long who = __ballot(spoilt >> i & 1); who; who &= who - 1) {
                     const int l = __builtin_ctzll(who);
-                    const float v = half_bits_to_float(vb[(size_t)(4 * l + i) * rows + base + j]);
+                    const float v = half_bits_to_float(vb[(size_t)(__shfl(e, l) + i) * rows + base + j]);
                     const float sum = wave_pairwise_sum(sees ? p * v : 0.0f);
                     if (lane == l)
                         o[i] += sum;
@@ -364,22 +384,285 @@ __device__ __forceinline__ v4f attn_tree_again(const Args &x, const Tree &t, int
     return o;
 }
 
+// Four elements' results at `at`: the quotients, and the Q8_0 of 32 elements by
+// the eight lanes that hold them.
+__device__ __forceinline__ void attn_tree_store(const Args &x, v4f o, bool any, float l, size_t at) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        y[i] = any ? o[i] / l : 0.0f;
+    if (x.out && ((uintptr_t)x.out & 15) == 0)
+        *(v4f *)(x.out + at) = v4f{y[0], y[1], y[2], y[3]};
+    else if (x.out)
+        for (int i = 0; i < 4; i++)
+            x.out[at + i] = y[i];
+    if (x.q8) {
+        float stored;
+        int32_t sm;
+        const uint32_t packed = q8_0_quad(y, &stored, &sm);
+        if (((uintptr_t)x.q8 & 3) == 0)
+            *(uint32_t *)(x.q8 + at) = packed;
+        else
+            for (int i = 0; i < 4; i++)
+                x.q8[at + i] = (int8_t)(packed >> (8 * i));
+        if ((threadIdx.x & 7) == 0) {
+            x.scales[at >> 5] = stored;
+            x.qsum[at >> 5] = sm;
+        }
+    }
+}
+
+// A tree whose rows are one tile: eight wavefronts of a workgroup take steps of
+// 32 keys in turn, each with its own maximum and sum, keys and values straight
+// into registers (no other tile wants them): the next step's keys asked for
+// before this one's products, its values as soon as this one's are used.  The
+// wavefronts' results are added in LDS.  Where one workgroup covers the keys (S
+// 1) it writes the results itself, and there is no join.  grid (kv_heads, 1,
+// trees * S).
+//
+// Bound by the loads: 64 trees of five nodes over 2000 positions (8 key-value
+// heads, 128 wide) read 524 MB in 103 us, 5.1 TB/s; one tree over 32000 takes
+// 38 us with its join, eight over 1500 take 17 where the kernel for more tiles
+// takes 21, 32 over 500 take 16 where it takes 23, and one over 60 takes 7
+// where it and the join take 10.
+template <int HD>
+__global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
+    constexpr int KS = HD / 16, ET = HD / 32, W = 8;
+    __shared__ __align__(16) float lds[W * kTile * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 31, h = lane >> 5;
+    const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
+    const Tree t(x, b, kNarrow);
+    const int g = x.heads / x.kv_heads, R = t.T * g;  // at most a tile
+    const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
+    if (R == 0 || t0 >= t1)
+        return;
+    const int slot = __builtin_amdgcn_readfirstlane(x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0);
+    const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
+    const uint16_t *kc = x.kc + cache, *vc = x.vc + cache;
+    const uint16_t *kd = x.kd + (size_t)kvh * HD * x.draft_context, *vd = x.vd + (size_t)kvh * HD * x.draft_context;
+    const int swapped = (li & ~12) | ((li & 4) << 1) | ((li & 8) >> 1);
+
+    // step j's rows: where they begin, and which of them there are
+    auto rows_of = [&](int j, int &p0, int &lo, int &hi) __attribute__((always_inline)) {
+        const bool draft = j >= t.np;
+        p0 = draft ? t.f0 - t.a + kNarrow * (j - t.np) : kNarrow * j;
+        lo = draft ? t.f0 : 0;
+        hi = draft ? t.f0 + t.T : t.P;
+        return draft;
+    };
+    v8h a0[KS], a1[KS], v[2][ET];
+    auto load_keys = [&](int j, v8h *a) __attribute__((always_inline)) {
+        int p0, lo, hi;
+        const bool draft = rows_of(j, p0, lo, hi);
+        const int rows = draft ? x.draft_context : x.context;
+        const char *kb = (const char *)(draft ? kd : kc);
+        const uint32_t at = ((uint32_t)h * rows + min(max(p0 + swapped, lo), hi - 1)) * 16;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+            a[k] = *(const v8h *)(kb + (size_t)(2 * k) * rows * 16 + at);
+    };
+    auto load_values = [&](int j) __attribute__((always_inline)) {
+        int p0, lo, hi;
+        const bool draft = rows_of(j, p0, lo, hi);
+        const int rows = draft ? x.draft_context : x.context;
+        const char *vb = (const char *)(draft ? vd : vc);
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            const int c = min(max(p0 + 16 * w + 8 * h, lo & ~7), (hi - 1) & ~7);
+            const uint32_t at = ((uint32_t)li * rows + c) * 2;
+#pragma unroll
+            for (int et = 0; et < ET; et++)
+                v[w][et] = *(const v8h *)(vb + (size_t)(32 * et) * rows * 2 + at);
+        }
+    };
+    const int r = min(li, R - 1), node = r / g;
+    v16f o[ET] = {};
+    float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
+    int j = t0 + wave;
+    if (j < t1) {
+        load_keys(j, a0);
+        const uint16_t *qr = x.qh + ((size_t)(t.f0 + node) * x.heads + kvh * g + (r - node * g)) * HD + 8 * h;
+        v8h q[KS];
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+            q[s] = *(const v8h *)(qr + 16 * s);
+        // (a tile's trees have at most 32 nodes: one mask word)
+        const uint32_t word = x.mask[t.f0 + node] & (uint32_t)((1ull << t.T) - 1);
+        load_values(j);
+        reads_first();
+        auto step = [&](v8h *a, v8h *an) __attribute__((always_inline)) {
+            const bool more = j + W < t1;
+            if (more)
+                load_keys(j + W, an);
+            reads_first();
+            v16f s = {}, s1 = {};
+#pragma unroll
+            for (int k = 0; k < KS; k += 2) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k], q[k], s, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k + 1], q[k + 1], s1, 0, 0, 0);
+            }
+            s += s1;
+            int p0, lo, hi;
+            const bool draft = rows_of(j, p0, lo, hi);
+            if (draft || p0 + kNarrow > hi) {
+                // bit k of sees: key k of the step; values past the rows there are become zero
+                const uint32_t sees = draft ? (uint32_t)(((uint64_t)word << t.a) >> (kNarrow * (j - t.np)))
+                                            : (1u << (hi - p0)) - 1;
+                const uint32_t bits = sees >> (8 * h);
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    s[i] = bits >> (16 * (i >> 3) + (i & 7)) & 1 ? s[i] : -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    const int c = min(max(p0 + 16 * w + 8 * h, lo & ~7), (hi - 1) & ~7);
+#pragma unroll
+                    for (int et = 0; et < ET; et++)
+                        v[w][et] = keep(v[w][et], lo - c, hi - c);
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                mx = fmaxf(mx, s[i]);
+            mx = halves_max(mx);
+            if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
+                const float mn = fmaxf(m, mx);
+                const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        o[et][i] *= corr;
+            }
+            const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                v8h ph, pl;
+                chances(s, w, x.c, base, ph, pl, l);
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+                    o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], ph, o[et], 0, 0, 0);
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+                    o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], pl, o[et], 0, 0, 0);
+            }
+            if (more)
+                load_values(j + W);
+            reads_first();
+        };
+        for (;;) {
+            step(a0, a1);
+            if ((j += W) >= t1)
+                break;
+            step(a1, a0);
+            if ((j += W) >= t1)
+                break;
+        }
+        l += __shfl_xor(l, 32);
+    }
+    // the wavefronts' maxima and sums, then their outputs times their weights, 64
+    // elements a round: a row's sixteen pieces exchanged by its low bits, without
+    // conflicts both ways
+    if (h == 0) {
+        lds[wave * kTile + li] = m;
+        lds[(W + wave) * kTile + li] = l;
+    }
+    __syncthreads();
+    const int row = tid >> 4, piece = tid & 15;  // what this thread adds up
+    const int had = min(W, t1 - t0);             // wavefronts that had a step
+    float top = -INFINITY, mine = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        top = fmaxf(top, lds[w * kTile + row]);
+        mine = fmaxf(mine, lds[w * kTile + li]);
+    }
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        // (a wavefront that saw nothing, or nothing but NaN, has no maximum)
+        const float mw = lds[w * kTile + row], lw = lds[(W + w) * kTile + row];
+        sum += mw == -INFINITY ? lw : lw * __builtin_amdgcn_exp2f((mw - top) * x.c);
+    }
+    const float weight = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mine) * x.c);
+    constexpr int kRounds = (ET + 1) / 2;
+    v4f y[kRounds];
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) {
+        __syncthreads();
+        float *to = lds + (wave * kTile + li) * 64;
+        if (wave < had)
+#pragma unroll
+            for (int e2 = 0; e2 < 2 && 2 * k + e2 < ET; e2++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v4f z;
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        z[u] = weight == 0.0f ? 0.0f : o[2 * k + e2][4 * i + u] * weight;
+                    *(v4f *)(to + 4 * ((8 * e2 + 2 * i + h) ^ (li & 15))) = z;
+                }
+        __syncthreads();
+        y[k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (64 * k + 4 * piece < HD)
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const v4f z = *(const v4f *)(lds + (w * kTile + row) * 64 + 4 * (piece ^ (row & 15)));
+                y[k] += w < had ? z : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+    }
+    const bool there = row < R;
+    const int tn = min(row, R - 1) / g, tok = t.f0 + tn, head = kvh * g + (min(row, R - 1) - tn * g);
+    if (x.S > 1) {
+        const size_t part = ((size_t)sp * x.M + tok) * x.heads + head;
+#pragma unroll
+        for (int k = 0; k < kRounds; k++)
+            if (there && 64 * k + 4 * piece < HD)
+                *(v4f *)(x.po + part * HD + 64 * k + 4 * piece) = y[k];
+        if (there && piece == 0) {
+            x.pml[2 * part] = top == -INFINITY ? top : top * x.c;
+            x.pml[2 * part + 1] = sum;
+        }
+        return;
+    }
+    const bool any = t.P > 0 || (x.mask[tok] & (uint32_t)((1ull << t.T) - 1)) != 0;
+#pragma unroll
+    for (int k = 0; k < kRounds; k++) {
+        const int e = 64 * k + 4 * piece;
+        uint32_t spoilt = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (there && e < HD && any && sum - sum == 0.0f && y[k][i] - y[k][i] != 0.0f)
+                spoilt |= 1u << i;
+        for (unsigned long long who = __ballot(spoilt != 0); who;) {  // a row after another
+            const int first = __builtin_ctzll(who) & ~15;
+            const uint32_t here = (lane & ~15) == first ? spoilt : 0u;
+            y[k] = attn_tree_again<HD>(x, t, b, __builtin_amdgcn_readlane(tok, first),
+                                       __builtin_amdgcn_readlane(head, first),
+                                       __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), first)) * x.c,
+                                       y[k], e, here);
+            who &= ~(0xFFFFull << first);
+        }
+        if (there && e < HD)
+            attn_tree_store(x, y[k], any, sum, ((size_t)tok * x.heads + head) * HD + e);
+    }
+}
+
 // A row (a node's head) a wavefront: its shares' maxima and sums a lane each,
 // its outputs four elements a lane, several shares side by side, added in a
 // fixed order; and the Q8_0 of 32 elements.  grid (heads / 4, M), 256 threads.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float *__restrict__ out,
-                                                             int8_t *__restrict__ q8, float *__restrict__ scales,
-                                                             int32_t *__restrict__ qsum) {
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x) {
     constexpr int L = HD / 4, SP = 64 / L;  // lanes a share, shares side by side
-    const int lane = threadIdx.x & 63, tok = blockIdx.y, width = x.heads * HD;
+    const int lane = threadIdx.x & 63, tok = blockIdx.y;
     const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head >= x.heads)
         return;
     int b = x.n == 1 ? 0 : -1;  // the tree: the last whose first token is not past this one
     for (int i = 0; x.n > 1 && i < x.n; i += 64)
         b += __popcll(__ballot(i + lane < x.n && x.first[min(i + lane, x.n - 1)] <= tok));
-    const Tree t(x, max(b, 0));
+    const Tree t(x, max(b, 0), x.stage);
     if (b < 0 || tok < t.f0 || tok >= t.f0 + t.T)
         return;
     const int live = (t.total + t.per - 1) / t.per;  // at most 64
@@ -430,34 +713,10 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x, float
         if (lane < L && any && l - l == 0.0f && o[i] - o[i] != 0.0f)
             spoilt |= 1u << i;
     if (__ballot(spoilt != 0))
-        o = attn_tree_again<HD>(x, t, b, tok, head, top, o, spoilt);
+        o = attn_tree_again<HD>(x, t, b, tok, head, top, o, e, spoilt);
     if (lane >= L)
         return;
-    v4f y;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        y[i] = any ? o[i] / l : 0.0f;
-    const size_t at = (size_t)tok * width + head * HD + e;
-    if (out && ((uintptr_t)out & 15) == 0)
-        *(v4f *)(out + at) = y;
-    else if (out)
-        for (int i = 0; i < 4; i++)
-            out[at + i] = y[i];
-    if (q8) {
-        const float v[4] = {y[0], y[1], y[2], y[3]};
-        float stored;
-        int32_t sm;
-        const uint32_t packed = q8_0_quad(v, &stored, &sm);
-        if (((uintptr_t)q8 & 3) == 0)
-            *(uint32_t *)(q8 + at) = packed;
-        else
-            for (int i = 0; i < 4; i++)
-                q8[at + i] = (int8_t)(packed >> (8 * i));
-        if ((lane & 7) == 0) {
-            scales[at >> 5] = stored;
-            qsum[at >> 5] = sm;
-        }
-    }
+    attn_tree_store(x, o, any, l, (size_t)tok * x.heads * HD + head * HD + e);
 }
 
 // Wavefronts a workgroup: a group's tiles of rows, the groups alike.
@@ -470,25 +729,45 @@ struct Groups {
     }
 };
 
+// One tile of rows a tree.
+bool narrow(int max_nodes, int heads, int kv_heads) { return max_nodes * (heads / kv_heads) <= kTile; }
+
 // Shares of the keys: as many workgroups as run at once (two wavefronts a SIMD
 // by their registers, two workgroups a CU by their LDS), so that the last round
-// is whole.
+// is whole (512 of more than four wavefronts: 82 us where 256 take 70).  Of one
+// tile a tree: one share, and no join, up to two steps a wavefront (250
+// positions 9.4 us, and 9.8 in shares; 500 positions 11.8 so, and 10.0 in
+// shares); past that two steps a share while there are CUs (four: 10.5 for the
+// 10.0; sixteen: 12.2), and 512 workgroups instead of 256 take 46 us over
+// 32000 positions where these take 38.
 int splits(int n, int max_nodes, int heads, int kv_heads, int max_prefix) {
+    const int64_t trees = (int64_t)std::max(n, 1) * kv_heads;
+    if (narrow(max_nodes, heads, kv_heads)) {
+        const int steps = (max_prefix + kNarrow - 1) / kNarrow + (max_nodes + 7 + kNarrow - 1) / kNarrow;
+        return steps <= 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(steps + 1) / 2, kMaxSplits, 256 / trees}));
+    }
     const Groups w(max_nodes, heads, kv_heads);
     const int steps = (max_prefix + kStage - 1) / kStage + (max_nodes + 7 + kStage - 1) / kStage;
-    const int64_t one = (int64_t)std::max(n, 1) * kv_heads * w.groups, most = w.waves > 4 ? 256 : 512;
+    const int64_t one = trees * w.groups, most = w.waves > 4 ? 256 : 512;
     return (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, most / one}));
 }
 
 template <int HD>
-int launch_hd(gx_ctx *ctx, const Args &x, float *out, int8_t *q, float *scales, int32_t *qsum) {
-    const Groups w(x.max_nodes, x.heads, x.kv_heads);
-    const dim3 grid((unsigned)x.kv_heads, (unsigned)w.groups, (unsigned)(x.n * x.S));
-    attn_tree_kernel<HD><<<grid, 64 * w.waves, 2 * 256 * HD, ctx->stream>>>(x);
+int launch_hd(gx_ctx *ctx, const Args &x) {
+    if (narrow(x.max_nodes, x.heads, x.kv_heads)) {
+        const dim3 grid((unsigned)x.kv_heads, 1, (unsigned)(x.n * x.S));
+        attn_tree_narrow_kernel<HD><<<grid, 512, 0, ctx->stream>>>(x);
+    } else {
+        const Groups w(x.max_nodes, x.heads, x.kv_heads);
+        const dim3 grid((unsigned)x.kv_heads, (unsigned)w.groups, (unsigned)(x.n * x.S));
+        attn_tree_kernel<HD><<<grid, 64 * w.waves, 2 * 256 * HD, ctx->stream>>>(x);
+    }
     if (int rc = check_launch("attention of drafted trees"))
         return rc;
+    if (narrow(x.max_nodes, x.heads, x.kv_heads) && x.S == 1)
+        return GX_OK;
     const dim3 join((unsigned)((x.heads + 3) / 4), (unsigned)x.M);
-    attn_tree_join_kernel<HD><<<join, 256, 0, ctx->stream>>>(x, out, q, scales, qsum);
+    attn_tree_join_kernel<HD><<<join, 256, 0, ctx->stream>>>(x);
     return check_launch("attention of drafted trees, joined");
 }
 
@@ -507,16 +786,18 @@ int launch_attn_tree(gx_ctx *ctx, const TreeAttention &y, float *out, int8_t *q,
                  y.kcache,  y.vcache,  y.kdraft,    y.vdraft,  y.n,
                  y.M,       y.max_nodes, (y.max_nodes + 31) / 32, y.max_prefix, y.heads,
                  y.kv_heads, y.context, y.draft_context, y.nslots, S,
-                 (float)(1.4426950408889634 / sqrt((double)y.hd)), po, po + (size_t)S * y.M * y.heads * y.hd};
+                 narrow(y.max_nodes, y.heads, y.kv_heads) ? kNarrow : kStage,
+                 (float)(1.4426950408889634 / sqrt((double)y.hd)), po, po + (size_t)S * y.M * y.heads * y.hd,
+                 out,       q,         scales,      qsum};
     switch (y.hd) {
     case 32:
-        return launch_hd<32>(ctx, x, out, q, scales, qsum);
+        return launch_hd<32>(ctx, x);
     case 64:
-        return launch_hd<64>(ctx, x, out, q, scales, qsum);
+        return launch_hd<64>(ctx, x);
     case 96:
-        return launch_hd<96>(ctx, x, out, q, scales, qsum);
+        return launch_hd<96>(ctx, x);
     case 128:
-        return launch_hd<128>(ctx, x, out, q, scales, qsum);
+        return launch_hd<128>(ctx, x);
     default:
         return fail(GX_ERR_UNSUPPORTED, "gx: attention supports head widths 32, 64, 96 and 128");
     }

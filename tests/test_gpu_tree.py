@@ -177,15 +177,15 @@ class Attention:
         return [vmax * (2 * (hd * dot + 4 * (top + 12)) * e + 2 * 2 ** -22 + 3 * n * e)
                 for hd, n in ((self.hd, count + 64), (self.hd ** 0.5, (count + 64) ** 0.5))]
 
-    def run(self, dev, max_prefix=None, q8=False, fill=77.0, lone=False, nslots=None):
+    def run(self, dev, max_prefix=None, q8=False, fill=77.0, lone=False, nslots=None, skew=0):
         M, width = self.M, self.heads * self.hd
         kc = self.k.reshape(self.nslots, self.kv, self.context, self.hd // 8, 8).transpose(0, 1, 3, 2, 4)
         kd = self.kd.reshape(self.kv, self.dctx, self.hd // 8, 8).transpose(0, 2, 1, 3)
         h = [dev.put(np.ascontiguousarray(x).view(np.int16)) for x in (
             self.q, kc, self.v.transpose(0, 1, 3, 2), kd, self.vd.transpose(0, 2, 1))]
         first, mask, prefix, slots = (dev.put(x) for x in (self.first, self.mask.view(np.int32), self.prefix, self.slots))
-        out = dev.full((M, width), fill)
-        q, sc, qs = (dev.full((M, width), 55, np.int8), dev.full((M, width // 32), 55.0),
+        out = dev.full((M * width + skew,), fill)[skew:]
+        q, sc, qs = (dev.full((M * width + skew,), 55, np.int8)[skew:].reshape(M, width), dev.full((M, width // 32), 55.0),
                      dev.full((M, width // 32), 55, np.int32)) if q8 else (None, None, None)
         mp = int(max(self.prefix.max(), 0)) if max_prefix is None else max_prefix
         size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", self.n, M, self.max_nodes, self.heads, self.kv,
@@ -253,8 +253,18 @@ def test_attention_large_scores(dev):
     Attention(16, [20], [700], 4, 2, 64, spread=60.0).check(dev)
 
 
-def test_attention_q8_form_is_the_floats(dev, orc):
-    a = Attention(17, [11, 30], [333, 60], 6, 2, 96, pad=2)
+@pytest.mark.parametrize("heads,kv,hd,prefix", [(4, 2, 32, 3), (32, 8, 128, 300), (4, 4, 96, 40), (8, 2, 128, 1500),
+                                                (8, 1, 64, 5000)])
+def test_attention_one_tile(dev, heads, kv, hd, prefix):
+    """Trees that fill a tile of rows, and fill it but for a few, beside empty ones and shorter prefixes."""
+    most = 32 * kv // heads
+    Attention(25, [most, 0, 1, max(most - 1, 1)], [prefix, 5, prefix // 2, 0], heads, kv, hd, pad=2).check(dev)
+    Attention(26, [1, most], [prefix, prefix + 9], heads, kv, hd, fanout=1, max_nodes=most).check(dev)
+
+
+@pytest.mark.parametrize("sizes,prefix", [([11, 30], [333, 60]), ([10, 3], [333, 60]), ([10, 3], [1333, 60])])
+def test_attention_q8_form_is_the_floats(dev, orc, sizes, prefix):
+    a = Attention(17, sizes, prefix, 6, 2, 96, pad=2)
     o, q, sc, qs = a.run(dev, q8=True)
     b = orc.Batch(np.ascontiguousarray(o[:a.tokens].reshape(a.tokens, -1))).quantize()
     np.testing.assert_array_equal(q[:a.tokens], b.q_rows())
@@ -262,6 +272,14 @@ def test_attention_q8_form_is_the_floats(dev, orc):
     np.testing.assert_array_equal(sc[:a.tokens], scale.astype(np.float16).astype(np.float32))
     np.testing.assert_array_equal(qs[:a.tokens], q[:a.tokens].reshape(a.tokens, -1, 32).sum(2, dtype=np.int32))
     assert np.all(q[a.tokens:] == 55) and np.all(sc[a.tokens:] == 55.0) and np.all(qs[a.tokens:] == 55)
+
+
+@pytest.mark.parametrize("prefix,max_nodes", [(70, None), (1100, None), (70, 64)])
+def test_attention_outputs_of_any_alignment(dev, prefix, max_nodes):
+    """Outputs off the alignment of their wide stores: floats by 4 bytes, bytes by 1."""
+    a = Attention(24, [7, 2], [prefix, 9], 4, 2, 64, max_nodes=max_nodes, pad=1)
+    for x, y in zip(a.run(dev, q8=True), a.run(dev, q8=True, skew=1)):
+        np.testing.assert_array_equal(x, y)
 
 
 def test_attention_masks_of_any_kind(dev):
@@ -276,14 +294,19 @@ def test_attention_masks_of_any_kind(dev):
     assert np.all(got[a.first[1] + 2] == 0) and np.all(got[a.first[2]:] == 0)
 
 
+# One tile's trees in one workgroup, over several, and as more tiles' trees.
+FORMS = [(70, None), (1100, None), (70, 64)]
+
+
+@pytest.mark.parametrize("prefix,max_nodes", FORMS)
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-def test_attention_hidden_values_stay_hidden(dev, bad):
+def test_attention_hidden_values_stay_hidden(dev, bad, prefix, max_nodes):
     """Infinite and NaN keys and values of nodes that a node does not see
     reach nothing of it; those it sees reach it as they would in float64.  An
     element that shares its tile with a hidden one is summed again key by key,
     another order of the same sum: within the same tolerance of the float64
     result; every other keeps its bits."""
-    a = Attention(20, [6, 5], [70, 9], 4, 2, 64, fanout=1)
+    a = Attention(20, [6, 5], [prefix, 9], 4, 2, 64, fanout=1, max_nodes=max_nodes)
     a.mask[:] = 0
     for b in range(2):
         for i in range(a.sizes[b]):  # nodes see themselves and the next but one before
@@ -305,8 +328,9 @@ def test_attention_hidden_values_stay_hidden(dev, bad):
     assert np.all(np.isnan(got[rows, 2:])) and np.all(np.isnan(want[rows, 2:]))
 
 
-def test_attention_infinite_cached_values(dev):
-    a = Attention(21, [3], [100], 4, 2, 64)
+@pytest.mark.parametrize("prefix,max_nodes", [(100, None), (1100, None), (100, 64)])
+def test_attention_infinite_cached_values(dev, prefix, max_nodes):
+    a = Attention(21, [3], [prefix], 4, 2, 64, max_nodes=max_nodes)
     a.v[a.slots[0], 0, 41, 5], a.v[a.slots[0], 1, 99, 0] = np.inf, -np.inf
     got, (want, tol) = a.run(dev), a.reference()
     fine = np.isfinite(want)
@@ -315,8 +339,9 @@ def test_attention_infinite_cached_values(dev):
     assert np.all(np.abs(got - np.where(fine, want, 0))[fine] <= np.broadcast_to(tol[..., :1], got.shape)[fine])
 
 
-def test_attention_nan_query_is_its_own(dev):
-    a = Attention(22, [9], [40], 4, 2, 64)
+@pytest.mark.parametrize("prefix,max_nodes", FORMS)
+def test_attention_nan_query_is_its_own(dev, prefix, max_nodes):
+    a = Attention(22, [9], [prefix], 4, 2, 64, max_nodes=max_nodes)
     clean = a.run(dev)
     a.q[4] = np.nan
     got = a.run(dev)
