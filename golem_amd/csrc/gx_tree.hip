@@ -230,16 +230,18 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
-// What a walk's workgroups share, one a tree.  The first of them walks; where
-// it needs a sum over a row it hands out the row's parts to whoever asks, the
-// others and itself, and waits for the parts that were taken: only ever for a
-// workgroup that runs.  The others wait only for one that walks: a workgroup
-// that finds none walking after a while ends, and so do all when the walk does.
+// What a walk's workgroups share, one a tree.  The first of them walks; the
+// others, once they have seen it walk, join it under a number each.  Where it
+// needs a sum over a row it says which in `what`, and how many had joined: they
+// and it take every so many-th of the row's parts, and it waits for theirs, so
+// only ever for a workgroup that runs and stays until the walk has ended.  The
+// others wait only for one that walks: a workgroup that finds none walking
+// after a while ends.
 struct Share {
-    unsigned long long claim;  // the sum's number in the high half, the next part in the low
-    // the open sum (six words: one load and one store of a wavefront's lanes): the
-    // row and the tokens turned down, then the row's largest logit and the factor
-    // of its exponentials in what is left, and the draft's
+    unsigned long long begun;                // 1 while the first walks
+    alignas(128) unsigned long long joined;  // the others that have joined
+    // the open sum: words that name it in their high 16 bits each, so that they need
+    // no order among them (one load and one store of a wavefront's lanes)
     alignas(128) unsigned long long what[8];
     // the parts' sums, kNone until they are there; odd and even sums apart, so that
     // the next one's can be cleared while this one's are on their way
@@ -247,8 +249,7 @@ struct Share {
     int gone[kTreeNodes];
 };
 constexpr unsigned long long kNone = ~0ull;  // (the bits of no sum: a logit's NaN has low bits of zero)
-// claims before the first sum and after the last (a late asker's count stays in the low half)
-constexpr unsigned long long kWalking = 1, kWalked = 0xFFFFFFFF00000000ull;
+constexpr int kWalked = 0xFFFF;              // what[0]'s name behind the last sum (0 before the first)
 
 template <typename T>
 __device__ __forceinline__ T share_load(const T *p) {
@@ -266,7 +267,7 @@ __device__ __forceinline__ T share_add(T *p, T v) {
 // Everything before it done, for every XCD, before anything after: all that the
 // workgroups share goes through the two calls above, past the caches that are
 // not coherent, so waiting for them is enough.  (Agent-scope release and acquire
-// would write back and drop the XCD's L2 each time: 20 us a sum in place of 5.)
+// would write back and drop the XCD's L2 each time: 20 us a sum in place of 7.)
 __device__ __forceinline__ void share_order() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // grid (chunks, M, 1 or 2): a chunk's largest logit and sum of exponentials,
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
     }
     if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0)
         for (int b = tid; b < n; b += kStatThreads)
-            share[b].claim = 0;
+            share[b].begun = share[b].joined = 0;
 }
 
 // grid (chunks, M): a chunk's largest logit and the lowest index that has it, by
@@ -401,16 +402,19 @@ struct Left {
     const int *gone;
     int turned, vocab;
     // eight tokens x0, x0 + step, ..; none past the vocabulary
-    __device__ __forceinline__ void eight(int x0, int step, double w[8]) const {
-        float l[8], d[8];
+    __device__ __forceinline__ void load(const float *from, int x0, int step, float v[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            l[i] = lr[min(x0 + i * step, vocab - 1)];
-        if (dr) {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                d[i] = dr[min(x0 + i * step, vocab - 1)];
-        }
+            v[i] = from[min(x0 + i * step, vocab - 1)];
+    }
+    __device__ __forceinline__ void eight(int x0, int step, double w[8]) const {
+        float l[8], d[8];
+        load(lr, x0, step, l);
+        if (dr)
+            load(dr, x0, step, d);
+        chances(x0, step, l, d, w);
+    }
+    __device__ __forceinline__ void chances(int x0, int step, const float l[8], const float d[8], double w[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             double r = p(l[i]) * scale;
@@ -425,61 +429,53 @@ struct Left {
     }
 };
 
-// One part's sum, by the whole workgroup (every thread gets it): eight tokens
-// a thread, a wavefront's 64 tokens in a row.
-__device__ __forceinline__ double part_sum(const Left &left, int k, double *wsum) {
-    const int tid = threadIdx.x;
-    double w[8];
-    left.eight(k * kPart + tid, kWalkThreads, w);
-    double s = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-    s = wave_sum64(s);
-    __syncthreads();
-    if ((tid & 63) == 0)
-        wsum[tid >> 6] = s;
-    __syncthreads();
-    s = wsum[0];
-    for (int i = 1; i < kWalkThreads / 64; i++)
-        s += wsum[i];
-    return s;
-}
-
-// The part of the open sum that `old`, a claim of this workgroup, names; false
-// where the claim came after the last.
-struct Helper {
+// A workgroup's parts of the sums of its tree.
+struct Parts {
     const WalkArgs &a;
-    Share &sh;
     const double *table;
     double *wsum;
-    unsigned long long *what;
-    int *gone;
-    int parts;
-    __device__ __forceinline__ bool one(unsigned long long old) {
-        const int tid = threadIdx.x, k = (int)(unsigned)old;
-        if (k >= parts)
-            return false;
-        if (tid < 8)
-            what[tid] = share_load(&sh.what[tid]);
-        __syncthreads();
-        const int row = (int)what[0], turned = (int)what[1];
-        const double dscale = __longlong_as_double((long long)what[5]);
-        if (turned > 0) {
-            for (int i = tid; i < turned; i += kWalkThreads)
-                gone[i] = share_load(&sh.gone[i]);
-            __syncthreads();
+    // the part that was loaded last, and its logits: a row's next sum is often of the
+    // same row, its chances scaled anew
+    float l[8], d[8];
+    int part = -1, target = -1, draft = -1;
+    __device__ __forceinline__ Left left(int row, int listed, const int *gone, double top, double dtop, double scale,
+                                         double dscale) const {
+        return Left{a.logits + (size_t)row * a.ldl,
+                    dscale > 0.0 ? a.draft + (size_t)row * a.ldd : nullptr,
+                    Exp64(table, a.it, top),
+                    Exp64(table, a.itd, dtop),
+                    scale,
+                    dscale,
+                    gone,
+                    listed,
+                    a.vocab};
+    }
+    // Part k's sum, by the whole workgroup (every thread gets it): eight tokens a
+    // thread, a wavefront's 64 tokens in a row.
+    __device__ __forceinline__ double sum(const Left &of, int row, int k) {
+        const int tid = threadIdx.x, x0 = k * kPart + tid;
+        if (part != k || target != row)
+            of.load(of.lr, x0, kWalkThreads, l);
+        if (of.dr && (part != k || draft != row)) {
+            of.load(of.dr, x0, kWalkThreads, d);
+            draft = row;
+        } else if (part != k) {
+            draft = -1;
         }
-        const Left left{a.logits + (size_t)row * a.ldl,
-                        dscale > 0.0 ? a.draft + (size_t)row * a.ldd : nullptr,
-                        Exp64(table, a.it, __longlong_as_double((long long)what[2])),
-                        Exp64(table, a.itd, __longlong_as_double((long long)what[4])),
-                        __longlong_as_double((long long)what[3]),
-                        dscale,
-                        gone,
-                        turned,
-                        a.vocab};
-        const double s = part_sum(left, k, wsum);
-        if (tid == 0)
-            share_store(&sh.part[old >> 32 & 1][k], (unsigned long long)__double_as_longlong(s));
-        return true;
+        part = k;
+        target = row;
+        double w[8];
+        of.chances(x0, kWalkThreads, l, d, w);
+        double s = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        s = wave_sum64(s);
+        __syncthreads();
+        if ((tid & 63) == 0)
+            wsum[tid >> 6] = s;
+        __syncthreads();
+        s = wsum[0];
+        for (int i = 1; i < kWalkThreads / 64; i++)
+            s += wsum[i];
+        return s;
     }
 };
 
@@ -499,7 +495,8 @@ __device__ __forceinline__ int first_of(int hit, int some, int *wmin) {
     return least <= kVocabMax ? least : 0x7ffffffe - least;
 }
 
-constexpr int kPolls = 400;  // looks for a walk that has begun, before a helper ends
+constexpr int kPolls = 400;  // looks for a walk that has begun, before a workgroup ends
+constexpr int kLooks = 16;   // looks of the walk for workgroups that have not joined it yet
 
 // grid (groups, n): a tree's first workgroup walks, the others help.
 __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArgs a) {
@@ -520,38 +517,57 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     const int f0 = min(max(a.first[b], 0), a.M), T = min(min(max(a.first[b + 1], f0), a.M) - f0, a.max_nodes);
     const int parts = (a.vocab + kPart - 1) / kPart;
     Share &sh = a.share[b];
-    Helper help{a, sh, table, wsum, what, gone, parts};
+    Parts mine{a, table, wsum};
     if (blockIdx.x > 0) {
         if (T <= 0)
             return;
         exp64_table(table);
-        int spent = 0;
-        for (;;) {
-            __syncthreads();
-            if (tid == 0) {
-                unsigned long long c;
-                for (;;) {
-                    c = share_load(&sh.claim);
-                    if (c >> 32 == kWalked >> 32)
-                        break;
-                    if (c == 0 && ++spent > kPolls) {
-                        c = kWalked;
-                        break;
-                    }
-                    if (c >> 32 && (unsigned)c < (unsigned)parts) {
-                        c = share_add(&sh.claim, 1ull);
-                        break;
-                    }
-                    __builtin_amdgcn_s_sleep(8);
+        if (tid == 0) {
+            got = 0;
+            for (int spent = 0; spent < kPolls; spent++) {
+                if (share_load(&sh.begun) != 0) {
+                    got = share_add(&sh.joined, 1ull) + 1;
+                    break;
                 }
-                got = c;
-                share_order();
+                __builtin_amdgcn_s_sleep(8);
+            }
+        }
+        __syncthreads();
+        const int number = (int)got;
+        if (number == 0)
+            return;
+        for (int seen = 0;;) {
+            if (wave == 0) {
+                unsigned long long w;
+                for (;;) {
+                    w = share_load(&sh.what[lane & 7]);
+                    const int name = (int)(w >> 48), first = __builtin_amdgcn_readfirstlane(name);
+                    if (first == kWalked || (first != seen && __ballot(name != first) == 0))
+                        break;
+                    __builtin_amdgcn_s_sleep(4);
+                }
+                if (lane < 8)
+                    what[lane] = w;
             }
             __syncthreads();
-            const unsigned long long mine = got;
-            if (mine >> 32 == kWalked >> 32)
+            const unsigned long long w0 = what[0];
+            seen = (int)(w0 >> 48);
+            if (seen == kWalked)
                 return;
-            help.one(mine);
+            const int row = (int)(w0 & 0xFFFF), listed = (int)(w0 >> 16 & 0x3FF), workers = (int)(w0 >> 26 & 0x3FF);
+            const Left left = mine.left(row, listed, gone, __uint_as_float((uint32_t)what[1]),
+                                        __uint_as_float((uint32_t)what[2]),
+                                        __hiloint2double((int)(uint32_t)what[4], (int)(uint32_t)what[3]),
+                                        __hiloint2double((int)(uint32_t)what[6], (int)(uint32_t)what[5]));
+            for (int i = tid; i < listed; i += kWalkThreads)
+                gone[i] = share_load(&sh.gone[i]);
+            __syncthreads();  // (and `what` has been read)
+            if (number < workers)
+                for (int k = number; k < parts; k += workers) {
+                    const double s = mine.sum(left, row, k);
+                    if (tid == 0)
+                        share_store(&sh.part[seen & 1][k], (unsigned long long)__double_as_longlong(s));
+                }
         }
     }
     int32_t *path = a.path + (size_t)b * a.max_nodes;
@@ -570,9 +586,13 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             share_store(&sh.part[parity][i], kNone);
     };
     if (!a.picks) {
-        if (tid == 0)
-            share_store(&sh.claim, kWalking);
         clear(1);
+        if (tid < 8)
+            share_store(&sh.what[tid], 0ull);
+        share_order();
+        __syncthreads();
+        if (tid == 0)
+            share_store(&sh.begun, 1ull);
     }
     exp64_table(table);
     for (int i = tid; i < T; i += kWalkThreads) {
@@ -658,6 +678,8 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         __syncthreads();
     }
+    if (tid == 0)
+        got = share_load(&sh.joined);
     for (int m = tid; m < T; m += kWalkThreads) {
         const int p = par[m], x = tok[m];
         if (p < 0 || p >= m || x < 0 || x >= a.vocab)
@@ -667,6 +689,16 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             qx[m] = Exp64(table, a.itd, dtop[p])(a.draft[(size_t)(f0 + p) * a.ldd + x]) / dsum[p];
     }
     __syncthreads();
+    // those that have joined, and this one (the others had time to since it began;
+    // what is left of them is waited for a little)
+    int workers = (int)got + 1;
+    for (int looks = 0; looks < kLooks && workers < a.groups; looks++) {
+        __syncthreads();
+        if (tid == 0)
+            got = share_load(&sh.joined);
+        __syncthreads();
+        workers = (int)got + 1;
+    }
     double c = 0.0, tried = 0.0, mass = 1.0, all = 0.0;
     int turned = 0, m = 1;
     unsigned sums = 0;
@@ -735,44 +767,48 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             // the sum of what is left of v's row, handed out
             const int listed = a.draft ? 0 : turned;
             sums++;
-            if (tid < 6) {
-                const double words[6] = {0.0, 0.0, top[v], 1.0 / sum[v], a.draft ? dtop[v] : 0.0, off()};
-                unsigned long long mine = tid == 0 ? (unsigned long long)(f0 + v) : (unsigned long long)listed;
-#pragma unroll
-                for (int i = 2; i < 6; i++)
-                    mine = tid == i ? (unsigned long long)__double_as_longlong(words[i]) : mine;
-                share_store(&sh.what[tid], mine);
-            }
             for (int i = tid; i < listed; i += kWalkThreads)
                 share_store(&sh.gone[i], gone[i]);
-            share_order();
+            share_order();  // (and the parts' sums are cleared)
             __syncthreads();
-            if (tid == 0) {
-                share_store(&sh.claim, (unsigned long long)sums << 32);
-                got = share_add(&sh.claim, 1ull);
+            const double scale = 1.0 / sum[v], dscale = off(), tv = top[v], dv = a.draft ? dtop[v] : 0.0;
+            if (tid < 8) {
+                const uint32_t words[8] = {0u,
+                                           __float_as_uint((float)tv),
+                                           __float_as_uint((float)dv),
+                                           (uint32_t)__double2loint(scale),
+                                           (uint32_t)__double2hiint(scale),
+                                           (uint32_t)__double2loint(dscale),
+                                           (uint32_t)__double2hiint(dscale),
+                                           0u};
+                unsigned long long mine = (unsigned long long)(f0 + v) | (unsigned long long)listed << 16 |
+                                          (unsigned long long)workers << 26;
+#pragma unroll
+                for (int i = 1; i < 8; i++)
+                    mine = tid == i ? words[i] : mine;
+                share_store(&sh.what[tid], mine | (unsigned long long)sums << 48);
             }
             clear((sums + 1) & 1);
+            const Left left = mine.left(f0 + v, listed, gone, tv, dv, scale, dscale);
+            for (int k = 0; k < parts; k += workers) {
+                const double s = mine.sum(left, f0 + v, k);
+                if (tid == 0)
+                    own[k] = s;
+            }
             __syncthreads();
-            help.one(got);
-            // the parts' sums, two of them a thread, as they come; where there are more
-            // parts than workgroups, or they are long in coming, another part itself
+            // the parts' sums, two of them a thread, as they come
             static_assert(kParts == 2 * kWalkThreads, "two parts a thread");
             const unsigned long long *from = sh.part[sums & 1] + 2 * tid;
-            unsigned long long w1 = 2 * tid < parts ? kNone : 0ull, w2 = 2 * tid + 1 < parts ? kNone : 0ull;
-            for (int looks = 1;; looks++) {
+            auto at_hand = [&](int k) __attribute__((always_inline)) {
+                return k >= parts ? 0ull : k % workers ? kNone : (unsigned long long)__double_as_longlong(own[k]);
+            };
+            unsigned long long w1 = at_hand(2 * tid), w2 = at_hand(2 * tid + 1);
+            do {
                 if (w1 == kNone)
                     w1 = share_load(from);
                 if (w2 == kNone)
                     w2 = share_load(from + 1);
-                if (!__syncthreads_or(w1 == kNone || w2 == kNone))
-                    break;
-                if (parts > a.groups || looks % 8 == 0) {
-                    if (tid == 0)
-                        got = share_add(&sh.claim, 1ull);
-                    __syncthreads();
-                    help.one(got);
-                }
-            }
+            } while (__syncthreads_or(w1 == kNone || w2 == kNone));
             const double one = __longlong_as_double((long long)w1), two = __longlong_as_double((long long)w2);
             double up = one + two;
             for (int d = 1; d < 64; d <<= 1) {
@@ -806,7 +842,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         break;
     }
     if (tid == 0)
-        share_store(&sh.claim, kWalked);
+        share_store(&sh.what[0], (unsigned long long)kWalked << 48);
     int token = -1;
     if (all > 0.0 && all - all == 0.0) {
         const double aim = (double)un[0] * all;
@@ -824,15 +860,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         // the part's running sum: eight tokens in a row a thread
         constexpr int kEach = kPart / kWalkThreads;
         static_assert(kEach == 8, "Left::eight");
-        const Left left{a.logits + (size_t)(f0 + v) * a.ldl,
-                        off() > 0.0 ? a.draft + (size_t)(f0 + v) * a.ldd : nullptr,
-                        Exp64(table, a.it, top[v]),
-                        Exp64(table, a.itd, a.draft ? dtop[v] : 0.0),
-                        1.0 / sum[v],
-                        off(),
-                        gone,
-                        a.draft ? 0 : turned,
-                        a.vocab};
+        const Left left = mine.left(f0 + v, a.draft ? 0 : turned, gone, top[v], a.draft ? dtop[v] : 0.0, 1.0 / sum[v], off());
         const int x0 = k * kPart + tid * kEach;
         double w[kEach], mine = 0.0;
         left.eight(x0, 1, w);
