@@ -585,23 +585,50 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         for (int i = tid; i < parts; i += kWalkThreads)
             share_store(&sh.part[parity][i], kNone);
     };
+    // what hangs on nothing but the tree's place, asked for together: its nodes, and
+    // the chunks' statistics that are staged first
+    constexpr int kMine = kTreeNodes / kWalkThreads, kCell = kCells / kWalkThreads;
+    const int rows = a.draft ? 2 * T : T, batch = max(1, kCells / a.chunks);
+    float ct[kCell];
+    double cs[kCell];
+    auto load_cells = [&](int r0) __attribute__((always_inline)) {
+        // (the target's rows of a tree follow one another, and so do the draft's)
+        const int c0 = r0 * a.chunks, split = T * a.chunks, last = min(r0 + batch, rows) * a.chunks - 1;
+#pragma unroll
+        for (int k = 0; k < kCell; k++) {
+            const int i = min(c0 + tid + k * kWalkThreads, last);
+            const size_t at = i < split ? (size_t)f0 * a.chunks + i : (size_t)(a.M + f0) * a.chunks + (i - split);
+            ct[k] = a.tops[at];
+            cs[k] = a.sums[at];
+        }
+    };
+    int up[kMine], id[kMine];
+    float number[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; k++) {
+        const int i = f0 + min(tid + k * kWalkThreads, T - 1);
+        up[k] = a.parents[i];
+        id[k] = a.tokens[i];
+        number[k] = a.picks ? 0.0f : a.uniforms[i];
+    }
     if (!a.picks) {
+        load_cells(0);
         clear(1);
         if (tid < 8)
             share_store(&sh.what[tid], 0ull);
-        share_order();
-        __syncthreads();
-        if (tid == 0)
-            share_store(&sh.begun, 1ull);
     }
     exp64_table(table);
-    for (int i = tid; i < T; i += kWalkThreads) {
-        par[i] = a.parents[f0 + i];
-        tok[i] = a.tokens[f0 + i];
-        if (!a.picks)
-            un[i] = a.uniforms[f0 + i];
-    }
+#pragma unroll
+    for (int k = 0; k < kMine; k++)
+        if (tid + k * kWalkThreads < T) {
+            par[tid + k * kWalkThreads] = up[k];
+            tok[tid + k * kWalkThreads] = id[k];
+            un[tid + k * kWalkThreads] = number[k];
+        }
+    share_order();
     __syncthreads();  // (and the path's -1s are written)
+    if (!a.picks && tid == 0)
+        share_store(&sh.begun, 1ull);
     if (tid == 0)
         path[0] = 0;
     int v = 0, kept = 1;
@@ -610,16 +637,15 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             const size_t row = f0 + i;
             float best = -INFINITY;
             int id = 0;
+            const float zero = a.logits[row * a.ldl];
             for (int c = lane; c < a.chunks; c += 64) {
                 const float v = a.tops[row * a.chunks + c];
-                if (v > best) {
-                    best = v;
-                    id = a.picks[row * a.chunks + c];
-                }
+                const int pick = a.picks[row * a.chunks + c];
+                id = v > best ? pick : id;
+                best = fmaxf(best, v);
             }
             const float mx = wave_max(best);
             id = wave_min_i32(best == mx && mx > -INFINITY ? id : 0x7fffffff);
-            const float zero = a.logits[row * a.ldl];
             if (lane == 0)
                 gone[i] = zero != zero || id == 0x7fffffff ? 0 : id;
         }
@@ -637,24 +663,22 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
         }
         return;
     }
-    // every row's statistics from its chunks' (staged in LDS, so many rows' at a
-    // time), then every child's chances
-    const int rows = a.draft ? 2 * T : T, batch = max(1, kCells / a.chunks);
+    // a child's logits in its parent's rows, and every row's statistics from its
+    // chunks' (staged in LDS, so many rows' at a time); then every child's chances
+    float lx[kMine], dx[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; k++) {
+        const int m = min(tid + k * kWalkThreads, T - 1), p = min(max(par[m], 0), T - 1);
+        const int x = min(max(tok[m], 0), a.vocab - 1);
+        lx[k] = a.logits[(size_t)(f0 + p) * a.ldl + x];
+        dx[k] = a.draft ? a.draft[(size_t)(f0 + p) * a.ldd + x] : 0.0f;
+    }
     for (int r0 = 0; r0 < rows; r0 += batch) {
         const int here = min(batch, rows - r0);
-        // (the target's rows of a tree follow one another, and so do the draft's)
-        const int c0 = r0 * a.chunks, split = T * a.chunks, last = (r0 + here) * a.chunks - 1;
-        float ct[kCells / kWalkThreads];
-        double cs[kCells / kWalkThreads];
+        if (r0 > 0)
+            load_cells(r0);
 #pragma unroll
-        for (int k = 0; k < kCells / kWalkThreads; k++) {
-            const int i = min(c0 + tid + k * kWalkThreads, last);
-            const size_t at = i < split ? (size_t)f0 * a.chunks + i : (size_t)(a.M + f0) * a.chunks + (i - split);
-            ct[k] = a.tops[at];
-            cs[k] = a.sums[at];
-        }
-#pragma unroll
-        for (int k = 0; k < kCells / kWalkThreads; k++) {
+        for (int k = 0; k < kCell; k++) {
             ctop[tid + k * kWalkThreads] = ct[k];
             csum[tid + k * kWalkThreads] = cs[k];
         }
@@ -680,13 +704,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
     }
     if (tid == 0)
         got = share_load(&sh.joined);
-    for (int m = tid; m < T; m += kWalkThreads) {
-        const int p = par[m], x = tok[m];
-        if (p < 0 || p >= m || x < 0 || x >= a.vocab)
+#pragma unroll
+    for (int k = 0; k < kMine; k++) {
+        const int m = tid + k * kWalkThreads, p = m < T ? par[m] : -1;
+        if (p < 0 || p >= m || tok[m] < 0 || tok[m] >= a.vocab)
             continue;
-        px[m] = Exp64(table, a.it, top[p])(a.logits[(size_t)(f0 + p) * a.ldl + x]) / sum[p];
+        px[m] = Exp64(table, a.it, top[p])(lx[k]) / sum[p];
         if (a.draft)
-            qx[m] = Exp64(table, a.itd, dtop[p])(a.draft[(size_t)(f0 + p) * a.ldd + x]) / dsum[p];
+            qx[m] = Exp64(table, a.itd, dtop[p])(dx[k]) / dsum[p];
     }
     __syncthreads();
     // those that have joined, and this one (the others had time to since it began;
