@@ -25,6 +25,7 @@
 // compute and take attn_tree_narrow_kernel; where their prefixes are short that
 // is the only launch.  Larger trees take attn_tree_kernel.
 #include <algorithm>
+#include <type_traits>
 
 #include "gx_device.hpp"
 #include "gx_internal.hpp"
@@ -54,7 +55,7 @@ struct Args {
     const int32_t *prefix;
     const int32_t *slots;
     const uint16_t *kc, *vc, *kd, *vd;
-    int n, M, max_nodes, words, max_prefix, heads, kv_heads, context, draft_context, nslots, S, stage;
+    int n, M, max_nodes, words, max_prefix, heads, kv_heads, context, draft_context, nslots, S, stage, halves;
     float c;       // 1 / sqrt(hd) in the exponent's base 2
     float *po;     // [S][M][heads][hd] unnormalised outputs
     float *pml;    // [S][M][heads][2] maximum (base 2) and sum
@@ -154,7 +155,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const int nw = blockDim.x >> 6, li = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
     const Tree t(x, b, kStage);
-    const int g = x.heads / x.kv_heads, R = t.T * g, g0 = blockIdx.y * nw * kTile, r0 = g0 + wave * kTile;
+    // Five or six tiles: the first four a wavefront each, the others two, one of
+    // each step's halves each, so that no SIMD has two whole tiles (eight trees of
+    // 33 nodes over 4000 positions 46 us, and 51 with five whole ones; of 80, 81 and 91).
+    const int tiles = x.halves ? nw / 2 + 2 : nw, whole = x.halves ? 4 : nw;
+    const int half = wave < whole ? 0 : (wave - whole) & 1, tile = wave < whole ? wave : whole + (wave - whole) / 2;
+    const int g = x.heads / x.kv_heads, R = t.T * g, g0 = blockIdx.y * tiles * kTile, r0 = g0 + tile * kTile;
     const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
     if (g0 >= R || t0 >= t1)
         return;
@@ -211,123 +217,167 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     v16f o[ET] = {};
     float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
     int at = 0;
-    for (int j = t0; j < t1; j++, at = kSlot - at) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();
-        if (j + 1 < t1)
-            load(j + 1, lds + (kSlot - at));
-        uint8_t *st = lds + at;
-        int p0, lo, hi;
-        const bool draft = rows_of(j, p0, lo, hi);
-        // Keys and chunks of values past the rows that there are repeat one that is
-        // (its chance will be zero); the rows beside those in a chunk become zero.
-        const int cl = p0 < lo ? (lo - p0) >> 3 : -1, ch = p0 + kStage > hi ? (hi - p0) >> 3 : -1;
-        if ((cl >= 0 && (lo & 7)) || (ch >= 0 && (hi & 7))) {
-            for (int e = tid; e < HD; e += 64 * nw) {
-                uint8_t *vr = st + HD * 128 + e * 128;
-                if (cl >= 0) {
-                    v8h *to = (v8h *)(vr + ((cl ^ (e & 7)) << 4));
-                    *to = keep(*to, lo - (p0 + 8 * cl), hi - (p0 + 8 * cl));
-                }
-                if (ch >= 0 && ch < 8) {
-                    v8h *to = (v8h *)(vr + ((ch ^ (e & 7)) << 4));
-                    *to = keep(*to, lo - (p0 + 8 * ch), hi - (p0 + 8 * ch));
-                }
-            }
+    // the steps, 32 U keys of each from the u0-th half on
+    auto steps = [&](auto count, int u0) __attribute__((always_inline)) {
+        constexpr int U = decltype(count)::value;
+        for (int j = t0; j < t1; j++, at = kSlot - at) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             lds_barrier();
-        }
-        if (r0 >= R)
-            continue;
-        v8h a[KS][2];
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                a[k][u] = *(const v8h *)(st + klane + 2048 * k + 512 * u);
-        reads_first();
-        v16f s[2] = {};
-#pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-                s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k][u], q[k], s[u], 0, 0, 0);
-        v8h v[4][ET];
-        auto values = [&](int w) __attribute__((always_inline)) {
-#pragma unroll
-            for (int et = 0; et < ET; et++)
-                v[w][et] = *(const v8h *)(st + vlane + 4096 * et + (((uint32_t)(2 * w) ^ vx) << 4));
-        };
-        values(0);
-        values(1);
-        reads_first();
-        if (draft || p0 + kStage > hi) {
-            // bit k of sees[u]: key 32 u + k of the step
-            const int above = hi - p0, below = max(lo - p0, 0);
-            uint32_t sees[2];
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int n = min(max(above - 32 * u, 0), 32), z = min(max(below - 32 * u, 0), 32);
-                sees[u] = (uint32_t)((1ull << n) - (1ull << z)) & (n > z ? ~0u : 0u);
+            if (j + 1 < t1)
+                load(j + 1, lds + (kSlot - at));
+            uint8_t *st = lds + at;
+            int p0, lo, hi;
+            const bool draft = rows_of(j, p0, lo, hi);
+            // Keys and chunks of values past the rows that there are repeat one that is
+            // (its chance will be zero); the rows beside those in a chunk become zero.
+            const int cl = p0 < lo ? (lo - p0) >> 3 : -1, ch = p0 + kStage > hi ? (hi - p0) >> 3 : -1;
+            if ((cl >= 0 && (lo & 7)) || (ch >= 0 && (hi & 7))) {
+                for (int e = tid; e < HD; e += 64 * nw) {
+                    uint8_t *vr = st + HD * 128 + e * 128;
+                    if (cl >= 0) {
+                        v8h *to = (v8h *)(vr + ((cl ^ (e & 7)) << 4));
+                        *to = keep(*to, lo - (p0 + 8 * cl), hi - (p0 + 8 * cl));
+                    }
+                    if (ch >= 0 && ch < 8) {
+                        v8h *to = (v8h *)(vr + ((ch ^ (e & 7)) << 4));
+                        *to = keep(*to, lo - (p0 + 8 * ch), hi - (p0 + 8 * ch));
+                    }
+                }
+                lds_barrier();
             }
-            if (draft) {
-                const int w0 = 2 * (j - t.np);  // bits from node 32 w0 - a on
-                if (w0 > 0) {
+            if (r0 >= R)
+                continue;
+            v8h a[KS][U];
 #pragma unroll
-                    for (int i = 0; i < 3; i++)
-                        mw[i] = w0 + i <= x.words ? mrow[w0 + i - 1] : 0u;
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    a[k][u] = *(const v8h *)(st + klane + 2048 * k + 512 * (u0 + u));
+            reads_first();
+            v16f s[U] = {};
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k][u], q[k], s[u], 0, 0, 0);
+            v8h v[2 * U][ET];
+            auto values = [&](int w) __attribute__((always_inline)) {
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+                    v[w][et] = *(const v8h *)(st + vlane + 4096 * et + (((uint32_t)(2 * (2 * u0 + w)) ^ vx) << 4));
+            };
+            values(0);
+            values(1);
+            reads_first();
+            if (draft || p0 + kStage > hi) {
+                // bit k of sees[u]: key 32 (u0 + u) + k of the step
+                const int above = hi - p0, below = max(lo - p0, 0);
+                uint32_t sees[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int n = min(max(above - 32 * (u0 + u), 0), 32), z = min(max(below - 32 * (u0 + u), 0), 32);
+                    sees[u] = (uint32_t)((1ull << n) - (1ull << z)) & (n > z ? ~0u : 0u);
+                }
+                if (draft) {
+                    const int w0 = 2 * (j - t.np);  // bits from node 32 w0 - a on
+                    if (w0 > 0) {
+#pragma unroll
+                        for (int i = 0; i < 3; i++)
+                            mw[i] = w0 + i <= x.words ? mrow[w0 + i - 1] : 0u;
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t here = U == 1 && u0 ? mw[2] : mw[u + 1], last = U == 1 && u0 ? mw[1] : mw[u];
+                        sees[u] &= t.a ? (here << t.a) | (last >> (32 - t.a)) : here;
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-                    sees[u] &= t.a ? (mw[u + 1] << t.a) | (mw[u] >> (32 - t.a)) : mw[u + 1];
-            }
+                for (int u = 0; u < U; u++) {
+                    const uint32_t bits = sees[u] >> (8 * h);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const uint32_t bits = sees[u] >> (8 * h);
+                    for (int i = 0; i < 16; i++)
+                        s[u][i] = bits >> (16 * (i >> 3) + (i & 7)) & 1 ? s[u][i] : -INFINITY;
+                }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    s[u][i] = bits >> (16 * (i >> 3) + (i & 7)) & 1 ? s[u][i] : -INFINITY;
+                    mx = fmaxf(mx, s[u][i]);
+            mx = halves_max(mx);
+            // (a row that sees nothing yet, or whose maximum has risen past what the
+            // reference allows: the reference becomes the maximum)
+            if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
+                const float mn = fmaxf(m, mx);
+                const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        o[et][i] *= corr;
+            }
+            const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
+            v8h ph[2 * U], pl[2 * U];
+            chances(s[0], 0, x.c, base, ph[0], pl[0], l);
+#pragma unroll
+            for (int w = 0; w < 2 * U; w++) {
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+                    o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], ph[w], o[et], 0, 0, 0);
+#pragma unroll
+                for (int et = 0; et < ET; et++)
+                    o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], pl[w], o[et], 0, 0, 0);
+                if (w + 2 < 2 * U)
+                    values(w + 2);
+                if (w + 1 < 2 * U)
+                    chances(s[(w + 1) >> 1], (w + 1) & 1, x.c, base, ph[w + 1], pl[w + 1], l);
             }
         }
-        float mx = -INFINITY;
+    };
+    // (the loops meet at the same barriers)
+    if (x.halves && wave >= whole)
+        steps(std::integral_constant<int, 1>(), half);
+    else
+        steps(std::integral_constant<int, 2>(), 0);
+    l += __shfl_xor(l, 32);
+    if (x.halves) {  // a tile's second half joins its first
+        lds_barrier();
+        v4f *to = (v4f *)lds + (wave - whole) / 2 * (ET * 4 * 64) + lane;
+        float *const ml = (float *)(lds + kSlot) + (wave - whole) / 2 * 128 + lane;
+        if (wave >= whole && half) {
 #pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                mx = fmaxf(mx, s[u][i]);
-        mx = halves_max(mx);
-        // (a row that sees nothing yet, or whose maximum has risen past what the
-        // reference allows: the reference becomes the maximum)
-        if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
-            const float mn = fmaxf(m, mx);
-            const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+            for (int k = 0; k < 4 * ET; k++)
+                to[64 * k] = v4f{o[k / 4][4 * (k % 4)], o[k / 4][4 * (k % 4) + 1], o[k / 4][4 * (k % 4) + 2],
+                                 o[k / 4][4 * (k % 4) + 3]};
+            ml[0] = m;
+            ml[64] = l;
+        }
+        lds_barrier();
+        if (half)
+            return;
+        if (wave >= whole) {
+            const float m2 = ml[0], l2 = ml[64], mn = fmaxf(m, m2);
+            const float c1 = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+            const float c2 = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m2 - mn) * x.c);
+            // (a half that saw nothing, or nothing but NaN, has no maximum)
+            l = (m == -INFINITY ? l : l * c1) + (m2 == -INFINITY ? l2 : l2 * c2);
             m = mn;
-            l *= corr;
 #pragma unroll
-            for (int et = 0; et < ET; et++)
+            for (int k = 0; k < 4 * ET; k++) {
+                const v4f z = to[64 * k];
 #pragma unroll
-                for (int i = 0; i < 16; i++)
-                    o[et][i] *= corr;
-        }
-        const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
-        v8h ph[4], pl[4];
-        chances(s[0], 0, x.c, base, ph[0], pl[0], l);
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-#pragma unroll
-            for (int et = 0; et < ET; et++)
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], ph[w], o[et], 0, 0, 0);
-#pragma unroll
-            for (int et = 0; et < ET; et++)
-                o[et] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[w][et], pl[w], o[et], 0, 0, 0);
-            if (w < 2)
-                values(w + 2);
-            if (w < 3)
-                chances(s[(w + 1) >> 1], (w + 1) & 1, x.c, base, ph[w + 1], pl[w + 1], l);
+                for (int i = 0; i < 4; i++) {
+                    const float y = o[k / 4][4 * (k % 4) + i];
+                    o[k / 4][4 * (k % 4) + i] = (c1 == 0.0f ? 0.0f : y * c1) + (c2 == 0.0f ? 0.0f : z[i] * c2);
+                }
+            }
         }
     }
     if (r0 + li >= R)
         return;
-    l += __shfl_xor(l, 32);
     const size_t row = ((size_t)sp * x.M + t.f0 + node) * x.heads + kvh * g + (r - node * g);
     float *po = x.po + row * HD + 4 * h;
 #pragma unroll
@@ -721,11 +771,14 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x) {
 
 // Wavefronts a workgroup: a group's tiles of rows, the groups alike.
 struct Groups {
-    int waves, groups;
+    int waves, groups, halves;
     Groups(int max_nodes, int heads, int kv_heads) {
         const int tiles = (max_nodes * (heads / kv_heads) + kTile - 1) / kTile;
         groups = (tiles + kMaxWaves - 1) / kMaxWaves;
         waves = (tiles + groups - 1) / groups;
+        halves = waves == 5 || waves == 6;  // (the kernel's `tiles` from its wavefronts)
+        if (halves)
+            waves = 2 * waves - 4;
     }
 };
 
@@ -787,6 +840,7 @@ int launch_attn_tree(gx_ctx *ctx, const TreeAttention &y, float *out, int8_t *q,
                  y.M,       y.max_nodes, (y.max_nodes + 31) / 32, y.max_prefix, y.heads,
                  y.kv_heads, y.context, y.draft_context, y.nslots, S,
                  narrow(y.max_nodes, y.heads, y.kv_heads) ? kNarrow : kStage,
+                 Groups(y.max_nodes, y.heads, y.kv_heads).halves,
                  (float)(1.4426950408889634 / sqrt((double)y.hd)), po, po + (size_t)S * y.M * y.heads * y.hd,
                  out,       q,         scales,      qsum};
     switch (y.hd) {

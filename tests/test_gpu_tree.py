@@ -328,6 +328,30 @@ def test_attention_hidden_values_stay_hidden(dev, bad, prefix, max_nodes):
     assert np.all(np.isnan(got[rows, 2:])) and np.all(np.isnan(want[rows, 2:]))
 
 
+@pytest.mark.parametrize("heads,hd,nodes", [(4, 64, 80), (8, 128, 47), (2, 32, 190)])
+def test_attention_tiles_in_halves(dev, heads, hd, nodes):
+    """Trees of five and six tiles of rows, the last ones by halves of each
+    step: prefixes that end in either half, a NaN query and hidden NaN and
+    infinite values in the last tile."""
+    for prefix in (0, 20, 40, 64, 333):
+        Attention(27, [nodes, 3], [prefix, 50], heads, heads // 4 if heads > 4 else heads // 2, hd).check(dev)
+    a = Attention(28, [nodes], [77], heads, heads // 4 if heads > 4 else heads // 2, hd)
+    clean = a.run(dev)
+    a.q[nodes - 2] = np.nan
+    a.vd[:, nodes - 1] = np.nan
+    a.vd[0, nodes - 3, 5] = np.inf
+    seen = [nodes - 3 in a.sees(0, i) for i in range(nodes)]
+    got, (want, tol) = a.run(dev), a.reference()
+    assert np.all(np.isnan(got[nodes - 2:]))
+    group = heads // a.kv
+    for i in range(nodes - 2):
+        off = np.zeros((heads, hd), bool)
+        off[:group, 5] = seen[i]
+        assert np.all(got[i][off] == np.inf)
+        assert np.all(np.abs(got[i][~off] - want[i][~off]) <= np.broadcast_to(tol[i, :, :1], off.shape)[~off])
+    assert np.isfinite(clean).all() and not all(seen)
+
+
 @pytest.mark.parametrize("prefix,max_nodes", [(100, None), (1100, None), (100, 64)])
 def test_attention_infinite_cached_values(dev, prefix, max_nodes):
     a = Attention(21, [3], [prefix], 4, 2, 64, max_nodes=max_nodes)
