@@ -37,8 +37,12 @@ __global__ __launch_bounds__(256) void cache_commit_kernel(const CommitLayers at
     const size_t to = ((size_t)slot * kv_heads + kvh) * hd * context, src = (size_t)kvh * hd * draft_context;
     // Consecutive threads take consecutive positions of an element (or of a piece
     // of the keys), whose bytes lie together on both sides; all of a thread's
-    // loads before its stores.  (An element's positions a thread: each store on
-    // a line of its own, 74 us where this takes 38 for sixteen paths of twelve.)
+    // loads before its stores, the values' past the caches (kept there, sixteen
+    // paths of twelve through 36 layers take 45 us where this takes 37; the keys'
+    // past them too 42).  Bound by the stores' pieces: 24 bytes of values and 192
+    // of keys lie together, 69 MB move where 44 are wanted.  (An element's
+    // positions a thread: each store on a line of its own, 74 us; two positions a
+    // word a thread: 46.)
     v4u_stream *kc = (v4u_stream *)(at.kc[layer] + to);
     const v4u_stream *kd = (const v4u_stream *)(at.kd[layer] + src);
     uint16_t *vc = at.vc[layer] + to;
@@ -67,7 +71,7 @@ __global__ __launch_bounds__(256) void cache_commit_kernel(const CommitLayers at
 #pragma unroll
         for (int u = 0; u < 8; u++)
             if (vrow[u] >= 0)
-                vc[vpos[u]] = v[u];
+                __builtin_nontemporal_store(v[u], vc + vpos[u]);
     }
 }
 
