@@ -82,7 +82,9 @@ struct ForkLayers {
 
 // grid (kv_heads * hd / 8, 2, layers): a piece row of the keys (y 0, 16 bytes a
 // position) or eight element rows of the values (32 threads each).  Four loads
-// a thread before their stores.
+// a thread before their stores, and one read for all the copies.  At the rate of
+// a large copy (4.8 TB/s): 301 positions of 36 layers, 89 MB, in 16 us and four
+// copies of 1999, 1.47 GB, in 310.
 __global__ __launch_bounds__(256) void cache_fork_kernel(const ForkLayers at, int kv_heads, int hd, int context,
                                                          int src, int n, int len) {
     const int tid = threadIdx.x, layer = blockIdx.z;
