@@ -278,7 +278,9 @@ __device__ __forceinline__ void share_order() { asm volatile("s_waitcnt vmcnt(0)
 
 // grid (chunks, M, 1 or 2): a chunk's largest logit and sum of exponentials,
 // of the target's rows (z 0) and the draft's; and the walks' shares cleared.
-// A chunk stays in registers between the two.  204 rows of 151936 (124 MB and 31
+// A chunk stays in registers between the two; the loads stay in the caches, for
+// the walks (past them: 30 us become 32 for eight chains, 54 become 55 for four
+// trees).  204 rows of 151936 (124 MB and 31
 // million exponentials of twelve float64 operations and five others): 26 us,
 // where the loads alone would take 18 and the operations about 13; 72 rows 13.
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float *__restrict__ logits, int ldl,
@@ -300,7 +302,7 @@ __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float 
         typedef float v4f __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int k = 0; k < kMine / 4; k++) {
-            const v4f w = __builtin_nontemporal_load((const v4f *)(x + c0) + tid + k * kStatThreads);
+            const v4f w = *((const v4f *)(x + c0) + tid + k * kStatThreads);
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 v[4 * k + i] = w[i];
@@ -811,8 +813,12 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(const WalkArg
             sums++;
             for (int i = tid; i < listed; i += kWalkThreads)
                 share_store(&sh.gone[i], gone[i]);
+            if (tid == 0 && workers < a.groups)  // (more of them may have joined)
+                got = share_load(&sh.joined);
             share_order();  // (and the parts' sums are cleared)
             __syncthreads();
+            if (workers < a.groups)
+                workers = (int)got + 1;
             const double scale = 1.0 / sum[v], dscale = off(), tv = top[v], dv = a.draft ? dtop[v] : 0.0;
             if (tid < 8) {
                 const uint32_t words[8] = {0u,
