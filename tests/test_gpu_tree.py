@@ -239,9 +239,10 @@ def test_attention_many_trees(dev):
     Attention(14, list(g.integers(1, 5, 130)), list(g.integers(0, 70, 130)), 2, 1, 32).check(dev)
 
 
-def test_attention_launched_for_a_longer_prefix(dev):
+@pytest.mark.parametrize("sizes,max_nodes", [([9, 4], 70), ([9, 4], 40), ([8, 4], None)])
+def test_attention_launched_for_a_longer_prefix(dev, sizes, max_nodes):
     """max_prefix above every prefix (a captured pass), and rows of more mask words than the trees need."""
-    a = Attention(15, [9, 4], [100, 3], 8, 2, 128, max_nodes=70)
+    a = Attention(15, sizes, [100, 3], 8, 2, 128, max_nodes=max_nodes)
     a.k = np.concatenate([a.k, np.full_like(a.k, np.nan)] * 20, 2)
     a.v = np.concatenate([a.v, np.full_like(a.v, np.nan)] * 20, 2)
     a.context = a.k.shape[2]
@@ -394,14 +395,15 @@ def test_attention_one_conversation_and_clamped_slots(dev):
     np.testing.assert_array_equal(got, a.run(dev, max_prefix=50))
 
 
-def test_attention_past_32_bits(dev):
+@pytest.mark.parametrize("max_nodes", [5, 64])
+def test_attention_past_32_bits(dev, max_nodes):
     """A conversation whose cache begins past 2^32 bytes (and 2^31 elements)."""
     kv, hd, ctx, nslots = 2, 64, 262144, 68
     n = nslots * kv * hd * ctx  # 2.3e9 elements
     t = dev.torch
     kc = t.zeros(n, dtype=t.float16, device="cuda").view(nslots, kv, hd // 8, ctx, 8)
     vc = t.zeros(n, dtype=t.float16, device="cuda").view(nslots, kv, hd, ctx)
-    a = Attention(24, [5], [300], 4, kv, hd)
+    a = Attention(24, [5], [300], 4, kv, hd, max_nodes=max_nodes)
     k, v = a.k[0, :, :300], a.v[0, :, :300]
     kc[-1, :, :, :300] = t.from_numpy(k.reshape(kv, 300, hd // 8, 8).transpose(0, 2, 1, 3).copy()).cuda()
     vc[-1, :, :, :300] = t.from_numpy(v.transpose(0, 2, 1).copy()).cuda()
@@ -410,9 +412,9 @@ def test_attention_past_32_bits(dev):
     first, mask, prefix, slot, q = (dev.put(x) for x in (a.first, a.mask.view(np.int32), a.prefix,
                                                          np.array([nslots - 1], np.int32), a.q.view(np.int16)))
     out = dev.full((5, 4 * hd), 0.0)
-    size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", 1, 5, 5, 4, kv, hd, 300)
+    size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", 1, 5, max_nodes, 4, kv, hd, 300)
     ws = dev.empty((size,), np.uint8)
-    capi.call("gx_qwen_attention_tree", dev.ctx.ptr, vp(q), 1, 5, 5, vp(first), vp(mask), vp(prefix), 300, 4, kv, hd,
+    capi.call("gx_qwen_attention_tree", dev.ctx.ptr, vp(q), 1, 5, max_nodes, vp(first), vp(mask), vp(prefix), 300, 4, kv, hd,
               vp(kc), vp(vc), ctx, vp(kd), vp(vd), a.dctx, vp(out), None, None, None, vp(ws), size, vp(slot), nslots)
     want, tol = a.reference()
     assert np.all(np.abs(dev.get(out).reshape(5, 4, hd) - want) <= tol[..., :1])
