@@ -22,8 +22,8 @@
 //
 // Two kernels and a join of the keys' shares.  Trees of one tile of rows (eight
 // nodes of four query heads a key-value head, say) move bytes more than they
-// compute and take attn_tree_narrow_kernel; where their prefixes are short that
-// is the only launch.  Larger trees take attn_tree_kernel.
+// compute and take attn_tree_narrow_kernel, and so do larger ones over short
+// prefixes; the shortest need no join.  The others take attn_tree_kernel.
 #include <algorithm>
 #include <type_traits>
 
@@ -462,13 +462,12 @@ __device__ __forceinline__ void attn_tree_store(const Args &x, v4f o, bool any, 
     }
 }
 
-// A tree whose rows are one tile: eight wavefronts of a workgroup take steps of
-// 32 keys in turn, each with its own maximum and sum, keys and values straight
-// into registers (no other tile wants them): the next step's keys asked for
-// before this one's products, its values as soon as this one's are used.  The
-// wavefronts' results are added in LDS.  Where one workgroup covers the keys (S
-// 1) it writes the results itself, and there is no join.  grid (kv_heads, 1,
-// trees * S).
+// A tile of a tree's rows: eight wavefronts of a workgroup take steps of 32 keys
+// in turn, each with its own maximum and sum, keys and values straight into
+// registers: the next step's keys asked for before this one's products, its
+// values as soon as this one's are used.  The wavefronts' results are added in
+// LDS.  Where one workgroup covers the keys (S 1) it writes the results itself,
+// and there is no join.  grid (kv_heads, tiles, trees * S).
 //
 // Bound by the loads: 64 trees of five nodes over 2000 positions (8 key-value
 // heads, 128 wide) read 524 MB in 103 us, 5.1 TB/s; one tree over 32000 takes
@@ -483,9 +482,9 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
     const int li = lane & 31, h = lane >> 5;
     const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
     const Tree t(x, b, kNarrow);
-    const int g = x.heads / x.kv_heads, R = t.T * g;  // at most a tile
+    const int g = x.heads / x.kv_heads, R = t.T * g, r0 = blockIdx.y * kTile;
     const int t0 = sp * t.per, t1 = min(t.total, t0 + t.per);
-    if (R == 0 || t0 >= t1)
+    if (r0 >= R || t0 >= t1)
         return;
     const int slot = __builtin_amdgcn_readfirstlane(x.slots ? min(max(x.slots[b], 0), x.nslots - 1) : 0);
     const size_t cache = ((size_t)slot * x.kv_heads + kvh) * HD * x.context;
@@ -526,7 +525,7 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
                 v[w][et] = *(const v8h *)(vb + (size_t)(32 * et) * rows * 2 + at);
         }
     };
-    const int r = min(li, R - 1), node = r / g;
+    const int r = min(r0 + li, R - 1), node = r / g;
     v16f o[ET] = {};
     float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
     int j = t0 + wave;
@@ -537,8 +536,8 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
 #pragma unroll
         for (int s = 0; s < KS; s++)
             q[s] = *(const v8h *)(qr + 16 * s);
-        // (a tile's trees have at most 32 nodes: one mask word)
-        const uint32_t word = x.mask[t.f0 + node] & (uint32_t)((1ull << t.T) - 1);
+        const uint32_t *mrow = x.mask + (size_t)(t.f0 + node) * x.words;
+        const uint32_t first = mrow[0];
         load_values(j);
         reads_first();
         auto step = [&](v8h *a, v8h *an) __attribute__((always_inline)) {
@@ -557,8 +556,13 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
             const bool draft = rows_of(j, p0, lo, hi);
             if (draft || p0 + kNarrow > hi) {
                 // bit k of sees: key k of the step; values past the rows there are become zero
-                const uint32_t sees = draft ? (uint32_t)(((uint64_t)word << t.a) >> (kNarrow * (j - t.np)))
-                                            : (1u << (hi - p0)) - 1;
+                uint32_t sees = hi - p0 >= kNarrow ? ~0u : (1u << (hi - p0)) - 1;
+                if (draft) {
+                    const int w = j - t.np;
+                    const uint32_t here = w == 0 ? first : w < x.words ? mrow[w] : 0u;
+                    const uint32_t last = w == 0 ? 0u : w == 1 ? first : mrow[w - 1];
+                    sees &= t.a ? (here << t.a) | (last >> (32 - t.a)) : here;
+                }
                 const uint32_t bits = sees >> (8 * h);
 #pragma unroll
                 for (int i = 0; i < 16; i++)
@@ -662,8 +666,8 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
                 y[k] += w < had ? z : v4f{0.0f, 0.0f, 0.0f, 0.0f};
             }
     }
-    const bool there = row < R;
-    const int tn = min(row, R - 1) / g, tok = t.f0 + tn, head = kvh * g + (min(row, R - 1) - tn * g);
+    const bool there = r0 + row < R;
+    const int rr = min(r0 + row, R - 1), tn = rr / g, tok = t.f0 + tn, head = kvh * g + (rr - tn * g);
     if (x.S > 1) {
         const size_t part = ((size_t)sp * x.M + tok) * x.heads + head;
 #pragma unroll
@@ -676,7 +680,9 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
         }
         return;
     }
-    const bool any = t.P > 0 || (x.mask[tok] & (uint32_t)((1ull << t.T) - 1)) != 0;
+    bool any = t.P > 0;
+    for (int w = 0; !any && 32 * w < t.T; w++)
+        any = (x.mask[(size_t)tok * x.words + w] & (t.T - 32 * w >= 32 ? ~0u : (1u << (t.T - 32 * w)) - 1)) != 0;
 #pragma unroll
     for (int k = 0; k < kRounds; k++) {
         const int e = 64 * k + 4 * piece;
@@ -785,33 +791,43 @@ struct Groups {
     }
 };
 
-// One tile of rows a tree.
-bool narrow(int max_nodes, int heads, int kv_heads) { return max_nodes * (heads / kv_heads) <= kTile; }
+// How a call's rows and keys are shared out.
+struct Shares {
+    bool narrow;  // attn_tree_narrow_kernel's
+    int tiles;    // of rows a tree
+    int S;        // shares of the keys
+};
 
-// Shares of the keys: as many workgroups as run at once (two wavefronts a SIMD
-// by their registers, two workgroups a CU by their LDS), so that the last round
-// is whole (512 of more than four wavefronts: 82 us where 256 take 70).  Of one
-// tile a tree: one share, and no join, up to two steps a wavefront (250
-// positions 9.4 us, and 9.8 in shares; 500 positions 11.8 so, and 10.0 in
-// shares); past that two steps a share while there are CUs (four: 10.5 for the
-// 10.0; sixteen: 12.2), and 512 workgroups instead of 256 take 46 us over
-// 32000 positions where these take 38.
-int splits(int n, int max_nodes, int heads, int kv_heads, int max_prefix) {
-    const int64_t trees = (int64_t)std::max(n, 1) * kv_heads;
-    if (narrow(max_nodes, heads, kv_heads)) {
-        const int steps = (max_prefix + kNarrow - 1) / kNarrow + (max_nodes + 7 + kNarrow - 1) / kNarrow;
-        return steps <= 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(steps + 1) / 2, kMaxSplits, 256 / trees}));
-    }
+// A tile a workgroup (narrow): one share, and no join, up to two steps a
+// wavefront (five nodes over 250 positions 9.4 us, and 9.8 in shares; 64 over 300
+// 10.1 and 11.5; five over 500 11.8 and 10.0); past that two steps a share while
+// there are CUs (four: 10.5 for the 10.0; sixteen: 12.2; two workgroups a CU 46 us
+// over 32000 positions where one takes 38).  Trees of more tiles read the keys
+// again for each, from the caches, which costs less than the other kernel's
+// workgroups of several tiles up to seven steps a wavefront: 64 nodes over 20
+// positions 7.6 us for 14.1, over 2000 15.8 for 20.1; eight trees of 30 over 800
+// 16.4 for 21.9; at seven twelve of 20 over 800 16.7 for 21.8 and one of 33 over
+// 10000 28.2 for 27.0; at eight twelve of twelve over 2000 40.4 for 29.4.
+// That kernel: as many workgroups as run at once (two wavefronts a SIMD by their
+// registers, two workgroups a CU by their LDS), so that the last round is whole
+// (512 of more than four wavefronts: 82 us where 256 take 70).
+Shares shares(int n, int max_nodes, int heads, int kv_heads, int max_prefix) {
+    const int tiles = (max_nodes * (heads / kv_heads) + kTile - 1) / kTile;
+    const int64_t trees = (int64_t)std::max(n, 1) * kv_heads, all = trees * tiles;
+    const int few = (max_prefix + kNarrow - 1) / kNarrow + (max_nodes + 7 + kNarrow - 1) / kNarrow;
+    const int64_t S = few <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>({(few + 1) / 2, kMaxSplits, 256 / all}));
+    if (tiles == 1 || (all * S + 255) / 256 * few <= 7 * 8 * S)
+        return {true, tiles, (int)S};
     const Groups w(max_nodes, heads, kv_heads);
     const int steps = (max_prefix + kStage - 1) / kStage + (max_nodes + 7 + kStage - 1) / kStage;
     const int64_t one = trees * w.groups, most = w.waves > 4 ? 256 : 512;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, most / one}));
+    return {false, tiles, (int)std::max<int64_t>(1, std::min<int64_t>({steps, kMaxSplits, most / one}))};
 }
 
 template <int HD>
-int launch_hd(gx_ctx *ctx, const Args &x) {
-    if (narrow(x.max_nodes, x.heads, x.kv_heads)) {
-        const dim3 grid((unsigned)x.kv_heads, 1, (unsigned)(x.n * x.S));
+int launch_hd(gx_ctx *ctx, const Args &x, const Shares &y) {
+    if (y.narrow) {
+        const dim3 grid((unsigned)x.kv_heads, (unsigned)y.tiles, (unsigned)(x.n * x.S));
         attn_tree_narrow_kernel<HD><<<grid, 512, 0, ctx->stream>>>(x);
     } else {
         const Groups w(x.max_nodes, x.heads, x.kv_heads);
@@ -820,7 +836,7 @@ int launch_hd(gx_ctx *ctx, const Args &x) {
     }
     if (int rc = check_launch("attention of drafted trees"))
         return rc;
-    if (narrow(x.max_nodes, x.heads, x.kv_heads) && x.S == 1)
+    if (y.narrow && x.S == 1)
         return GX_OK;
     const dim3 join((unsigned)((x.heads + 3) / 4), (unsigned)x.M);
     attn_tree_join_kernel<HD><<<join, 256, 0, ctx->stream>>>(x);
@@ -830,31 +846,32 @@ int launch_hd(gx_ctx *ctx, const Args &x) {
 }  // namespace
 
 size_t attn_tree_workspace(int n, int M, int max_nodes, int heads, int kv_heads, int hd, int max_prefix) {
-    const size_t rows = (size_t)splits(n, max_nodes, heads, kv_heads, max_prefix) * M * heads;
+    const size_t rows = (size_t)shares(n, max_nodes, heads, kv_heads, max_prefix).S * M * heads;
     return ((rows * (hd + 2) * 4) + 255) & ~(size_t)255;
 }
 
 int launch_attn_tree(gx_ctx *ctx, const TreeAttention &y, float *out, int8_t *q, float *scales, int32_t *qsum,
                      uint8_t *workspace) {
-    const int S = splits(y.n, y.max_nodes, y.heads, y.kv_heads, y.max_prefix);
+    const Shares how = shares(y.n, y.max_nodes, y.heads, y.kv_heads, y.max_prefix);
+    const int S = how.S;
     float *po = (float *)workspace;
     const Args x{y.qh,      y.first,   y.mask,      y.prefix,  y.slots,
                  y.kcache,  y.vcache,  y.kdraft,    y.vdraft,  y.n,
                  y.M,       y.max_nodes, (y.max_nodes + 31) / 32, y.max_prefix, y.heads,
                  y.kv_heads, y.context, y.draft_context, y.nslots, S,
-                 narrow(y.max_nodes, y.heads, y.kv_heads) ? kNarrow : kStage,
+                 how.narrow ? kNarrow : kStage,
                  Groups(y.max_nodes, y.heads, y.kv_heads).halves,
                  (float)(1.4426950408889634 / sqrt((double)y.hd)), po, po + (size_t)S * y.M * y.heads * y.hd,
                  out,       q,         scales,      qsum};
     switch (y.hd) {
     case 32:
-        return launch_hd<32>(ctx, x);
+        return launch_hd<32>(ctx, x, how);
     case 64:
-        return launch_hd<64>(ctx, x);
+        return launch_hd<64>(ctx, x, how);
     case 96:
-        return launch_hd<96>(ctx, x);
+        return launch_hd<96>(ctx, x, how);
     case 128:
-        return launch_hd<128>(ctx, x);
+        return launch_hd<128>(ctx, x, how);
     default:
         return fail(GX_ERR_UNSUPPORTED, "gx: attention supports head widths 32, 64, 96 and 128");
     }

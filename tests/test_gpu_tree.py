@@ -105,11 +105,18 @@ def test_plan_leaves_out_what_has_no_place(dev):
 # ---- attention -----------------------------------------------------------------
 
 
+def long_context(n, max_nodes, heads, kv):
+    """A context past which a call is for the kernel whose workgroups have several tiles, and a little more."""
+    tiles = n * kv * ((max_nodes * (heads // kv) + 31) // 32)
+    return 32 * (7 * 8 * max(min(64, 256 // tiles), 1) + 2)
+
+
 class Attention:
     """A case's arrays: caches of nslots conversations filled with NaN past
     each prefix, draft buffers filled with NaN past the last token."""
 
-    def __init__(self, seed, sizes, prefix, heads, kv, hd, fanout=3, nslots=None, pad=0, max_nodes=None, spread=2.0):
+    def __init__(self, seed, sizes, prefix, heads, kv, hd, fanout=3, nslots=None, pad=0, max_nodes=None, spread=2.0,
+                 long=False):
         g = synth.rng(seed)
         self.sizes, self.prefix = list(sizes), np.array(prefix, np.int32)
         self.heads, self.kv, self.hd = heads, kv, hd
@@ -131,6 +138,11 @@ class Attention:
             p = int(self.prefix[list(self.slots).index(s)]) if s in self.slots else 0
             self.k[s, :, p:], self.v[s, :, p:] = np.nan, np.nan
         self.kd[:, self.tokens:], self.vd[:, self.tokens:] = np.nan, np.nan
+        if long:  # a context, launched for in whole, that has the tiles of a tree side by side in a workgroup
+            short, self.context = self.context, long_context(self.n, self.max_nodes, heads, kv)
+            more = ((0, 0), (0, 0), (0, self.context - short), (0, 0))
+            self.k, self.v = (np.pad(x, more, constant_values=np.nan) for x in (self.k, self.v))
+        self.long = long
         self.first = offsets(sizes)
         parents = random_parents(g, sizes, fanout)
         self.mask = plan_reference(sizes, parents, self.prefix, 1 << 30, self.max_nodes, self.M)[2]
@@ -187,7 +199,7 @@ class Attention:
         out = dev.full((M * width + skew,), fill)[skew:]
         q, sc, qs = (dev.full((M * width + skew,), 55, np.int8)[skew:].reshape(M, width), dev.full((M, width // 32), 55.0),
                      dev.full((M, width // 32), 55, np.int32)) if q8 else (None, None, None)
-        mp = int(max(self.prefix.max(), 0)) if max_prefix is None else max_prefix
+        mp = max_prefix if max_prefix is not None else self.context if self.long else int(max(self.prefix.max(), 0))
         size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", self.n, M, self.max_nodes, self.heads, self.kv,
                              self.hd, mp)
         ws = dev.full((max(size, 256),), 0xFF, np.uint8)
@@ -210,6 +222,8 @@ class Attention:
         return got
 
 
+# A tile a workgroup that covers the keys, the keys over several, and several tiles a workgroup.
+FORMS = [(70, None, False), (1100, None, False), (70, 64, True)]
 HEADS = [(4, 2, 64), (8, 2, 32), (6, 2, 96), (8, 2, 128), (3, 3, 64), (16, 1, 128), (5, 1, 32), (32, 8, 128)]
 
 
@@ -219,19 +233,29 @@ def test_attention_heads(dev, heads, kv, hd, sizes, prefix):
     Attention(10, sizes, prefix, heads, kv, hd).check(dev)
 
 
+@pytest.mark.parametrize("heads,kv,hd", HEADS)
+@pytest.mark.parametrize("sizes,prefix", [([65], [0]), ([40, 1, 70], [64, 200, 31])])
+def test_attention_heads_of_long_contexts(dev, heads, kv, hd, sizes, prefix):
+    Attention(10, sizes, prefix, heads, kv, hd, long=True).check(dev)
+
+
 @pytest.mark.parametrize("prefix", [0, 1, 7, 8, 31, 32, 33, 63, 64, 65, 127, 128, 129, 500, 1023, 2050])
 def test_attention_prefixes(dev, prefix):
     Attention(11, [5, 9], [prefix, max(prefix - 3, 0)], 4, 2, 64).check(dev)
+    Attention(11, [5, 37], [prefix, max(prefix - 3, 0)], 4, 2, 64, long=True).check(dev)
 
 
 @pytest.mark.parametrize("sizes", [[31], [32], [33], [64, 2], [3, 64, 30], [100], [129, 5], [1] * 11, [0, 4, 0, 3]])
 def test_attention_trees(dev, sizes):
     g = synth.rng(12)
-    Attention(12, sizes, list(g.integers(0, 90, len(sizes))), 4, 2, 64, nslots=len(sizes) + 2, pad=3).check(dev)
+    prefix = list(g.integers(0, 90, len(sizes)))
+    for long in (False, True):
+        Attention(12, sizes, prefix, 4, 2, 64, nslots=len(sizes) + 2, pad=3, long=long).check(dev)
 
 
 def test_attention_chain_of_512(dev):
-    Attention(13, [512], [40], 2, 1, 32, fanout=1).check(dev)
+    for long in (False, True):
+        Attention(13, [512], [40], 2, 1, 32, fanout=1, long=long).check(dev)
 
 
 def test_attention_many_trees(dev):
@@ -239,7 +263,7 @@ def test_attention_many_trees(dev):
     Attention(14, list(g.integers(1, 5, 130)), list(g.integers(0, 70, 130)), 2, 1, 32).check(dev)
 
 
-@pytest.mark.parametrize("sizes,max_nodes", [([9, 4], 70), ([9, 4], 40), ([8, 4], None)])
+@pytest.mark.parametrize("sizes,max_nodes", [([9, 4], 70), ([9, 4], 40), ([8, 4], None), ([9, 4], 512)])
 def test_attention_launched_for_a_longer_prefix(dev, sizes, max_nodes):
     """max_prefix above every prefix (a captured pass), and rows of more mask words than the trees need."""
     a = Attention(15, sizes, [100, 3], 8, 2, 128, max_nodes=max_nodes)
@@ -251,7 +275,8 @@ def test_attention_launched_for_a_longer_prefix(dev, sizes, max_nodes):
 
 def test_attention_large_scores(dev):
     """Scores of hundreds: one key takes all, as the maximum moves from tile to tile."""
-    Attention(16, [20], [700], 4, 2, 64, spread=60.0).check(dev)
+    for long in (False, True):
+        Attention(16, [20], [700], 4, 2, 64, spread=60.0, long=long).check(dev)
 
 
 @pytest.mark.parametrize("heads,kv,hd,prefix", [(4, 2, 32, 3), (32, 8, 128, 300), (4, 4, 96, 40), (8, 2, 128, 1500),
@@ -263,9 +288,10 @@ def test_attention_one_tile(dev, heads, kv, hd, prefix):
     Attention(26, [1, most], [prefix, prefix + 9], heads, kv, hd, fanout=1, max_nodes=most).check(dev)
 
 
-@pytest.mark.parametrize("sizes,prefix", [([11, 30], [333, 60]), ([10, 3], [333, 60]), ([10, 3], [1333, 60])])
-def test_attention_q8_form_is_the_floats(dev, orc, sizes, prefix):
-    a = Attention(17, sizes, prefix, 6, 2, 96, pad=2)
+@pytest.mark.parametrize("sizes,prefix,long", [([11, 30], [333, 60], False), ([11, 30], [333, 60], True),
+                                               ([10, 3], [333, 60], False), ([10, 3], [1333, 60], False)])
+def test_attention_q8_form_is_the_floats(dev, orc, sizes, prefix, long):
+    a = Attention(17, sizes, prefix, 6, 2, 96, pad=2, long=long)
     o, q, sc, qs = a.run(dev, q8=True)
     b = orc.Batch(np.ascontiguousarray(o[:a.tokens].reshape(a.tokens, -1))).quantize()
     np.testing.assert_array_equal(q[:a.tokens], b.q_rows())
@@ -275,17 +301,18 @@ def test_attention_q8_form_is_the_floats(dev, orc, sizes, prefix):
     assert np.all(q[a.tokens:] == 55) and np.all(sc[a.tokens:] == 55.0) and np.all(qs[a.tokens:] == 55)
 
 
-@pytest.mark.parametrize("prefix,max_nodes", [(70, None), (1100, None), (70, 64)])
-def test_attention_outputs_of_any_alignment(dev, prefix, max_nodes):
+@pytest.mark.parametrize("prefix,max_nodes,long", FORMS)
+def test_attention_outputs_of_any_alignment(dev, prefix, max_nodes, long):
     """Outputs off the alignment of their wide stores: floats by 4 bytes, bytes by 1."""
-    a = Attention(24, [7, 2], [prefix, 9], 4, 2, 64, max_nodes=max_nodes, pad=1)
+    a = Attention(24, [7, 2], [prefix, 9], 4, 2, 64, max_nodes=max_nodes, pad=1, long=long)
     for x, y in zip(a.run(dev, q8=True), a.run(dev, q8=True, skew=1)):
         np.testing.assert_array_equal(x, y)
 
 
-def test_attention_masks_of_any_kind(dev):
+@pytest.mark.parametrize("long", [False, True])
+def test_attention_masks_of_any_kind(dev, long):
     """Bits that are no tree's, bits past the tree's nodes, and nodes that see nothing."""
-    a = Attention(18, [40, 6, 3], [50, 0, 0], 4, 2, 64, max_nodes=64)
+    a = Attention(18, [40, 6, 3], [50, 0, 0], 4, 2, 64, max_nodes=64, long=long)
     g = synth.rng(19)
     a.mask[:] = g.integers(0, 1 << 32, a.mask.shape, dtype=np.uint64).astype(np.uint32)
     a.mask[a.first[1] + 2] = 0
@@ -295,19 +322,15 @@ def test_attention_masks_of_any_kind(dev):
     assert np.all(got[a.first[1] + 2] == 0) and np.all(got[a.first[2]:] == 0)
 
 
-# One tile's trees in one workgroup, over several, and as more tiles' trees.
-FORMS = [(70, None), (1100, None), (70, 64)]
-
-
-@pytest.mark.parametrize("prefix,max_nodes", FORMS)
+@pytest.mark.parametrize("prefix,max_nodes,long", FORMS)
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
-def test_attention_hidden_values_stay_hidden(dev, bad, prefix, max_nodes):
+def test_attention_hidden_values_stay_hidden(dev, bad, prefix, max_nodes, long):
     """Infinite and NaN keys and values of nodes that a node does not see
     reach nothing of it; those it sees reach it as they would in float64.  An
     element that shares its tile with a hidden one is summed again key by key,
     another order of the same sum: within the same tolerance of the float64
     result; every other keeps its bits."""
-    a = Attention(20, [6, 5], [prefix, 9], 4, 2, 64, fanout=1, max_nodes=max_nodes)
+    a = Attention(20, [6, 5], [prefix, 9], 4, 2, 64, fanout=1, max_nodes=max_nodes, long=long)
     a.mask[:] = 0
     for b in range(2):
         for i in range(a.sizes[b]):  # nodes see themselves and the next but one before
@@ -329,14 +352,16 @@ def test_attention_hidden_values_stay_hidden(dev, bad, prefix, max_nodes):
     assert np.all(np.isnan(got[rows, 2:])) and np.all(np.isnan(want[rows, 2:]))
 
 
+@pytest.mark.parametrize("long", [False, True])
 @pytest.mark.parametrize("heads,hd,nodes", [(4, 64, 80), (8, 128, 47), (2, 32, 190)])
-def test_attention_tiles_in_halves(dev, heads, hd, nodes):
+def test_attention_tiles_in_halves(dev, heads, hd, nodes, long):
     """Trees of five and six tiles of rows, the last ones by halves of each
     step: prefixes that end in either half, a NaN query and hidden NaN and
     infinite values in the last tile."""
+    kv = heads // 4 if heads > 4 else heads // 2
     for prefix in (0, 20, 40, 64, 333):
-        Attention(27, [nodes, 3], [prefix, 50], heads, heads // 4 if heads > 4 else heads // 2, hd).check(dev)
-    a = Attention(28, [nodes], [77], heads, heads // 4 if heads > 4 else heads // 2, hd)
+        Attention(27, [nodes, 3], [prefix, 50], heads, kv, hd, long=True).check(dev)
+    a = Attention(28, [nodes], [77], heads, kv, hd, long=long)
     clean = a.run(dev)
     a.q[nodes - 2] = np.nan
     a.vd[:, nodes - 1] = np.nan
@@ -353,9 +378,9 @@ def test_attention_tiles_in_halves(dev, heads, hd, nodes):
     assert np.isfinite(clean).all() and not all(seen)
 
 
-@pytest.mark.parametrize("prefix,max_nodes", [(100, None), (1100, None), (100, 64)])
-def test_attention_infinite_cached_values(dev, prefix, max_nodes):
-    a = Attention(21, [3], [prefix], 4, 2, 64, max_nodes=max_nodes)
+@pytest.mark.parametrize("prefix,max_nodes,long", [(100, None, False), (1100, None, False), (100, 64, True)])
+def test_attention_infinite_cached_values(dev, prefix, max_nodes, long):
+    a = Attention(21, [3], [prefix], 4, 2, 64, max_nodes=max_nodes, long=long)
     a.v[a.slots[0], 0, 41, 5], a.v[a.slots[0], 1, 99, 0] = np.inf, -np.inf
     got, (want, tol) = a.run(dev), a.reference()
     fine = np.isfinite(want)
@@ -364,9 +389,9 @@ def test_attention_infinite_cached_values(dev, prefix, max_nodes):
     assert np.all(np.abs(got - np.where(fine, want, 0))[fine] <= np.broadcast_to(tol[..., :1], got.shape)[fine])
 
 
-@pytest.mark.parametrize("prefix,max_nodes", FORMS)
-def test_attention_nan_query_is_its_own(dev, prefix, max_nodes):
-    a = Attention(22, [9], [prefix], 4, 2, 64, max_nodes=max_nodes)
+@pytest.mark.parametrize("prefix,max_nodes,long", FORMS)
+def test_attention_nan_query_is_its_own(dev, prefix, max_nodes, long):
+    a = Attention(22, [9], [prefix], 4, 2, 64, max_nodes=max_nodes, long=long)
     clean = a.run(dev)
     a.q[4] = np.nan
     got = a.run(dev)
@@ -395,8 +420,8 @@ def test_attention_one_conversation_and_clamped_slots(dev):
     np.testing.assert_array_equal(got, a.run(dev, max_prefix=50))
 
 
-@pytest.mark.parametrize("max_nodes", [5, 64])
-def test_attention_past_32_bits(dev, max_nodes):
+@pytest.mark.parametrize("max_nodes,max_prefix", [(5, 300), (64, 300), (64, 262144)])
+def test_attention_past_32_bits(dev, max_nodes, max_prefix):
     """A conversation whose cache begins past 2^32 bytes (and 2^31 elements)."""
     kv, hd, ctx, nslots = 2, 64, 262144, 68
     n = nslots * kv * hd * ctx  # 2.3e9 elements
@@ -412,10 +437,10 @@ def test_attention_past_32_bits(dev, max_nodes):
     first, mask, prefix, slot, q = (dev.put(x) for x in (a.first, a.mask.view(np.int32), a.prefix,
                                                          np.array([nslots - 1], np.int32), a.q.view(np.int16)))
     out = dev.full((5, 4 * hd), 0.0)
-    size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", 1, 5, max_nodes, 4, kv, hd, 300)
+    size = capi.size_out("gx_qwen_attention_tree_workspace_bytes", 1, 5, max_nodes, 4, kv, hd, max_prefix)
     ws = dev.empty((size,), np.uint8)
-    capi.call("gx_qwen_attention_tree", dev.ctx.ptr, vp(q), 1, 5, max_nodes, vp(first), vp(mask), vp(prefix), 300, 4, kv, hd,
-              vp(kc), vp(vc), ctx, vp(kd), vp(vd), a.dctx, vp(out), None, None, None, vp(ws), size, vp(slot), nslots)
+    capi.call("gx_qwen_attention_tree", dev.ctx.ptr, vp(q), 1, 5, max_nodes, vp(first), vp(mask), vp(prefix), max_prefix, 4, kv,
+              hd, vp(kc), vp(vc), ctx, vp(kd), vp(vd), a.dctx, vp(out), None, None, None, vp(ws), size, vp(slot), nslots)
     want, tol = a.reference()
     assert np.all(np.abs(dev.get(out).reshape(5, 4, hd) - want) <= tol[..., :1])
 
