@@ -281,8 +281,8 @@ __device__ __forceinline__ void share_order() { asm volatile("s_waitcnt vmcnt(0)
 // A chunk stays in registers between the two; the loads stay in the caches, for
 // the walks (past them: 30 us become 32 for eight chains, 54 become 55 for four
 // trees).  204 rows of 151936 (124 MB and 31
-// million exponentials of twelve float64 operations and five others): 26 us,
-// where the loads alone would take 18 and the operations about 13; 72 rows 13.
+// million exponentials of twelve float64 operations and five others): 25 us,
+// where the loads alone would take 18 and the operations about 13; 72 rows 12.
 __global__ __launch_bounds__(kStatThreads) void verify_stats_kernel(const float *__restrict__ logits, int ldl,
                                                                     const float *__restrict__ draft, int ldd,
                                                                     int vocab, double it, double itd,
@@ -513,7 +513,7 @@ constexpr int kLooks = 16;   // looks of the walk for workgroups that have not j
 // grid (groups, n): a tree's first workgroup walks, the others help.
 //
 // Bound by round trips to memory shared among the XCDs.  Eight chains of up to six
-// nodes over 151936 tokens take 18 us, four trees of up to 33 take 36: some 10 us to
+// nodes over 151936 tokens take 18 us, four trees of up to 33 take 37: some 10 us to
 // begin (the tree, its rows' sums, the children's chances, the others joining),
 // about 4 a sum, two loads and a scan to draw the last token.  A workgroup a tree
 // alone takes 360 and 590; parts handed out by a claim of each workgroup 20
