@@ -68,10 +68,11 @@ struct Args {
 // A tree's tokens, cached positions and steps, the same for every kernel.
 struct Tree {
     int f0, T, P, a, np, total, per;  // (total and per: steps)
-    __device__ Tree(const Args &x, int b, int stage) {
-        f0 = __builtin_amdgcn_readfirstlane(min(max(x.first[b], 0), x.M));
-        T = __builtin_amdgcn_readfirstlane(min(min(max(x.first[b + 1], f0), x.M) - f0, x.max_nodes));
-        P = __builtin_amdgcn_readfirstlane(min(max(x.prefix[b], 0), min(x.max_prefix, x.context)));
+    __device__ Tree(const Args &x, int b, int stage) : Tree(x, x.first[b], x.first[b + 1], x.prefix[b], stage) {}
+    __device__ Tree(const Args &x, int from, int to, int prefix, int stage) {
+        f0 = __builtin_amdgcn_readfirstlane(min(max(from, 0), x.M));
+        T = __builtin_amdgcn_readfirstlane(min(min(max(to, f0), x.M) - f0, x.max_nodes));
+        P = __builtin_amdgcn_readfirstlane(min(max(prefix, 0), min(x.max_prefix, x.context)));
         a = f0 & 7;  // draft rows are read from a multiple of 8
         np = (P + stage - 1) / stage;
         total = np + (T > 0 ? (a + T + stage - 1) / stage : 0);
@@ -708,7 +709,7 @@ __global__ __launch_bounds__(512) void attn_tree_narrow_kernel(const Args x) {
 // A row (a node's head) a wavefront: its shares' maxima and sums a lane each,
 // its outputs four elements a lane, several shares side by side, added in a
 // fixed order; and the Q8_0 of 32 elements.  grid (heads / 4, M), 256 threads.
-// Bound by its launch and two loads in a row for few rows (4.2 us for five nodes
+// Bound by its launch and loads for few rows (4.1 us for five nodes
 // of 32 heads in nine shares), by the shares' bytes for more (8.2 for 64 nodes in
 // 32 shares, 34 MB).
 template <int HD>
@@ -718,29 +719,39 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(const Args x) {
     const int head = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head >= x.heads)
         return;
-    int b = x.n == 1 ? 0 : -1;  // the tree: the last whose first token is not past this one
-    for (int i = 0; x.n > 1 && i < x.n; i += 64)
-        b += __popcll(__ballot(i + lane < x.n && x.first[min(i + lane, x.n - 1)] <= tok));
-    const Tree t(x, max(b, 0), x.stage);
-    if (b < 0 || tok < t.f0 || tok >= t.f0 + t.T)
-        return;
-    const int live = (t.total + t.per - 1) / t.per;  // at most 64
+    // All that hangs on the token alone is asked for together, whichever of the
+    // shares there are.
     const size_t row = (size_t)tok * x.heads + head, step = (size_t)x.M * x.heads;
     const int g = lane / L, e = 4 * (lane - g * L);
     typedef float v2f __attribute__((ext_vector_type(2)));
-    const v2f ml = *(const v2f *)(x.pml + (min(lane, live - 1) * step + row) * 2);
+    const v2f ml = *(const v2f *)(x.pml + (min(lane, x.S - 1) * step + row) * 2);
     const float *po = x.po + row * HD + e;
     auto shares = [&](int s0, v4f *p) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            p[k] = *(const v4f *)(po + (size_t)min(s0 + k * SP + g, live - 1) * step * HD);
+            p[k] = *(const v4f *)(po + (size_t)min(s0 + k * SP + g, x.S - 1) * step * HD);
     };
     v4f p[4];
     shares(0, p);
-    const uint32_t *mrow = x.mask + (size_t)tok * x.words;
-    const int bits = t.T - 32 * lane;  // nodes that this lane's mask word speaks of
-    const uint32_t word = bits > 0 ? mrow[lane] & (bits >= 32 ? ~0u : (1u << bits) - 1) : 0u;
-    reads_first();
+    const uint32_t seen = x.mask[(size_t)tok * x.words + min(lane, x.words - 1)];
+    int b = -1, from = 0, to = 0, prefix = 0;  // the tree: the last whose first token is not past this one
+    for (int i = 0; i < x.n; i += 64) {
+        const int k = min(i + lane, x.n - 1), f0 = x.first[k], f1 = x.first[k + 1], before = x.prefix[k];
+        reads_first();
+        const int count = __popcll(__ballot(i + lane < x.n && f0 <= tok));
+        if (count > 0) {
+            b = i + count - 1;
+            from = __builtin_amdgcn_readlane(f0, count - 1);
+            to = __builtin_amdgcn_readlane(f1, count - 1);
+            prefix = __builtin_amdgcn_readlane(before, count - 1);
+        }
+    }
+    const Tree t(x, from, to, prefix, x.stage);
+    if (b < 0 || tok < t.f0 || tok >= t.f0 + t.T)
+        return;
+    const int live = (t.total + t.per - 1) / t.per;  // at most S
+    const int bits = t.T - 32 * lane;                // nodes that this lane's mask word speaks of
+    const uint32_t word = bits > 0 ? seen & (bits >= 32 ? ~0u : (1u << bits) - 1) : 0u;
     const bool any = t.P > 0 || __ballot(word != 0) != 0;
     const float m = lane < live ? ml.x : -INFINITY, top = wave_max(m);
     const float weight = m == -INFINITY ? 0.0f : exp2f(m - top);
