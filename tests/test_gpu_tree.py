@@ -583,6 +583,16 @@ def test_verify(dev, sizes, fanout, V, pad, form):
     log(f"  {form}: the longest path keeps {longest}")
 
 
+@pytest.mark.parametrize("trees,V", [(300, 6000), (40, 40000), (700, 2049)])
+def test_verify_with_fewer_workgroups_than_parts(dev, trees, V):
+    """More trees than leave each one a workgroup for every part of its sums."""
+    sizes = [2] * trees
+    parents, tokens, logits, draft, u = make_verify(39, sizes, 1, V, True)
+    args = (sizes, parents, tokens, logits, draft, 1.0, 1.0, u, 2)
+    for x, y in zip(run_verify(dev, *args), verify_reference(*args)):
+        np.testing.assert_array_equal(x, y)
+
+
 def test_verify_temperatures_apart(dev):
     """A draft temperature of its own, and temperatures that leave one token or all alike."""
     sizes = [20, 9]
@@ -879,6 +889,25 @@ def test_speculation_draws_greedys_tokens(dev, width):
     m.reset()
     got, _ = m.speculate(prompt, steps, lambda ids: _oracle_draft(ids, prompt + want, width))
     assert got == want
+    m.free()
+
+
+def test_speculation_in_a_slot(dev):
+    """In one conversation of several, beside another whose caches stay as they are."""
+    m = _model(dev)
+    prompt, steps = [int(t) for t in synth.rng(66).integers(0, CFG.vocab, 7)], 24
+    want = m.greedy(prompt, steps)
+    m.set_slots(3)
+    m.use_slot(0)
+    m.forward([9, 8, 7], 0)
+    beside = [x[0].clone() for x in m.kc + m.vc]
+    m.use_slot(2)
+    got, passes = m.speculate(prompt, steps, lambda ids: _oracle_draft(ids, prompt + want, 2))
+    assert got == want and passes < steps // 2
+    for x, y in zip(beside, m.kc + m.vc):
+        assert torch.equal(x, y[0])
+    with pytest.raises(ValueError, match="exceed the context"):
+        m.speculate(prompt, m.slot_context, lambda ids: ([], []))
     m.free()
 
 
