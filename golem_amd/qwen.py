@@ -166,7 +166,7 @@ class QwenModel:
         self.slot_graphs = {}
         self.drafts = 0  # tokens the draft buffers hold (set_drafts)
         self.tree_ws, self.tree_ws_kept = None, []
-        self.tree_states = False  # the hidden states are forward_tree's
+        self.tree_states = False  # the tokens and hidden states are forward_tree's
         n = capi.size_out("gx_qwen_attention_workspace_bytes", M, cfg.heads, cfg.max_context - 1)
         self.attn_ws = torch.empty((n + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
         self._vp, self._call = vp, call
@@ -437,6 +437,7 @@ class QwenModel:
         if max(positions) >= self.slot_context:
             raise ValueError(f"qwen: position {max(positions)} is past a slot's {self.slot_context}")
         t = tokens if torch.is_tensor(tokens) else torch.tensor(np.asarray(tokens, dtype=np.int32))
+        self.tree_states = False  # their tokens are replaced
         self.tokens[:n].copy_(t)
         self.positions[:n].copy_(torch.tensor(np.asarray(positions, dtype=np.int32)))
         if self.nslots > 1:

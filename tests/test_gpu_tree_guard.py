@@ -1,0 +1,33 @@
+"""A pass over drafted tokens is judged by its own states and tokens or not at
+all: whatever replaces them in between is noticed."""
+import pytest
+import torch
+
+from tests.test_gpu_tree import _model
+
+pytestmark = pytest.mark.gpu
+
+
+def _drafted(dev):
+    m = _model(dev)
+    m.set_drafts(8)
+    m.forward([4, 5, 6], 0)
+    return m
+
+
+def _seed(x):
+    return torch.tensor([x], dtype=torch.int32, device="cuda")
+
+
+def test_seeding_lock_step_decoding_takes_the_drafts_away(dev):
+    """start_slots replaces the tokens that a verification compares with."""
+    m = _drafted(dev)
+    for tokens in ([9], _seed(9)):
+        m.forward_tree([[1, 2]], [[-1, 0]], [3])
+        m.start_slots(tokens, [3])
+        with pytest.raises(ValueError, match="another pass"):
+            m.verify_tree()
+        m.commit_tree()  # nothing verified: nothing to commit
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.verify_tree()
+    m.free()
