@@ -47,6 +47,7 @@ speculate is the loop over the three.
 """
 import ctypes
 import math
+import weakref
 
 import numpy as np
 import torch
@@ -91,6 +92,17 @@ class _Q8:
         self.q = torch.empty((M, K), dtype=torch.int8, device="cuda")
         self.s = torch.empty((M, K // 32), dtype=torch.float32, device="cuda")
         self.qs = torch.empty((M, K // 32), dtype=torch.int32, device="cuda")
+
+
+class _Step(torch.cuda.CUDAGraph):
+    """A model's captured step.  Every replay puts its own tokens and hidden
+    states in the place of those of a pass over drafted tokens."""
+
+    model = None  # a weak reference's proxy: the model holds its steps
+
+    def replay(self):
+        self.model.tree_states = False
+        super().replay()
 
 
 class QwenModel:
@@ -400,7 +412,8 @@ class QwenModel:
             raise ValueError("qwen: the captured decode step serves one conversation")
         torch.cuda.synchronize()
         stream = torch.cuda.Stream()
-        graph = torch.cuda.CUDAGraph()
+        graph = _Step()
+        graph.model = weakref.proxy(self)
         self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(stream.cuda_stream))
         try:
             with torch.cuda.graph(graph, stream=stream):
@@ -455,7 +468,6 @@ class QwenModel:
         top = max(self._slot_pos)
         if top >= self.slot_context:
             raise ValueError(f"qwen: position {top} is past a slot's {self.slot_context}")
-        self.tree_states = False
         if graph:
             self.capture_slots(n)
             self.slot_graphs[n].replay()
@@ -482,7 +494,8 @@ class QwenModel:
             raise ValueError(f"qwen: {n} conversations for {self.nslots} slots")
         torch.cuda.synchronize()
         stream = torch.cuda.Stream()
-        graph = torch.cuda.CUDAGraph()
+        graph = _Step()
+        graph.model = weakref.proxy(self)
         self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(stream.cuda_stream))
         try:
             with torch.cuda.graph(graph, stream=stream):
@@ -563,7 +576,7 @@ class QwenModel:
         also recorded as the history's entry `pos`."""
         if pos >= self.cfg.max_context:
             raise ValueError(f"qwen: position {pos} is past the context {self.cfg.max_context}")
-        self.tree_states = False
+        self.tree_states = False  # their tokens are replaced
         self.tokens[:1].copy_(tok)
         self.history[pos:pos + 1].copy_(tok)
         self.pos_dev.fill_(pos)
@@ -690,7 +703,8 @@ class QwenModel:
         the drafts being given tokens or, with draft_logits (device [M][vocab],
         the draft model's logits after each node), drawn from their softmax at
         draft_temperature (default: temperature).  No other pass may have run
-        since.  Returns device tensors:
+        since: the model's own are noticed and refused, replays of a graph that
+        a caller captured over them are not.  Returns device tensors:
         path [trees][nodes] (-1 behind), counts [trees], next [trees]."""
         t, vp, V = self._a_tree(), self._vp, self.cfg.vocab
         M = t["M"]

@@ -31,3 +31,26 @@ def test_seeding_lock_step_decoding_takes_the_drafts_away(dev):
     m.forward_tree([[1, 2]], [[-1, 0]], [3])
     m.verify_tree()
     m.free()
+
+
+def test_a_replayed_step_takes_the_drafts_away(dev):
+    """The captured decode step and the captured lock-step ones replace tokens
+    and hidden states at every replay, the first one after a pass over drafted
+    tokens included."""
+    m = _drafted(dev)
+    m.capture_decode()
+    m.start_decode(_seed(3), 5)
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.graph.replay()
+    with pytest.raises(ValueError, match="another pass"):
+        m.verify_tree()
+    m.set_slots(2)
+    m.start_slots([3, 4], [0, 0])
+    m.slots_step(2, graph=True)
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.slot_graphs[2].replay()
+    with pytest.raises(ValueError, match="another pass"):
+        m.verify_tree()
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.verify_tree()
+    m.free()
