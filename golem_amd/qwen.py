@@ -650,14 +650,17 @@ class QwenModel:
             return [x for row in v for x in row]
 
         first = np.concatenate([[0], np.cumsum(sizes)])
-        self.tokens[:M].copy_(dev(flat(tokens)))
-        self.tree = {"n": n, "M": M, "nodes": nodes, "first": dev(first), "parents": dev(flat(parents)),
-                     "prefix": dev(prefixes), "slots": dev(slots), "max_prefix": int(max(prefixes)),
-                     "mask": torch.empty((M, (nodes + 31) // 32), dtype=torch.int32, device="cuda"),
-                     "path": torch.full((n, nodes), -1, dtype=torch.int32, device="cuda"),
-                     "counts": torch.zeros((n,), dtype=torch.int32, device="cuda"),
-                     "next": torch.empty((n,), dtype=torch.int32, device="cuda")}
-        self._tree_blocks(self.tree)
+        ids = dev(flat(tokens))
+        tree = {"n": n, "M": M, "nodes": nodes, "first": dev(first), "parents": dev(flat(parents)),
+                "prefix": dev(prefixes), "slots": dev(slots), "max_prefix": int(max(prefixes)),
+                "mask": torch.empty((M, (nodes + 31) // 32), dtype=torch.int32, device="cuda"),
+                "path": torch.full((n, nodes), -1, dtype=torch.int32, device="cuda"),
+                "counts": torch.zeros((n,), dtype=torch.int32, device="cuda"),
+                "next": torch.empty((n,), dtype=torch.int32, device="cuda")}
+        self.tree = None  # none to judge until this one is whole
+        self.tokens[:M].copy_(ids)
+        self._tree_blocks(tree)
+        self.tree = tree
         return self.hidden[:M]
 
     def _tree_blocks(self, t):
@@ -667,7 +670,7 @@ class QwenModel:
         cfg, vp, call, ctx = self.cfg, self._vp, self._call, self.ctx.ptr
         n, M, nodes = t["n"], t["M"], t["nodes"]
         eps = np.float32(cfg.eps)
-        self.tree_states = True
+        self.tree_states = False
         call("gx_qwen_tree_plan", ctx, n, M, nodes, vp(t["first"]), vp(t["parents"]), vp(t["prefix"]),
              vp(self.rope_cos), vp(self.rope_sin), cfg.head_dim // 2, self.slot_context, vp(self.draft_rows),
              vp(self.positions), vp(t["mask"]), vp(self.draft_cos), vp(self.draft_sin))
@@ -694,6 +697,7 @@ class QwenModel:
             self._mm(b["down"], self.mid8, M, self.ffn, cfg.dim)
         call("gx_norm_quant", ctx, vp(self.xs), cfg.dim, vp(self.ffn), cfg.dim, vp(self.output_norm), M, cfg.dim,
              eps, vp(self.hidden), cfg.dim, None, None, None)
+        self.tree_states = True
 
     def verify_tree(self, temperature=0.0, draft_logits=None, draft_temperature=None, uniforms=None):
         """The walk down the trees of the last forward_tree by the target's

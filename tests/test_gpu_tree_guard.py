@@ -54,3 +54,34 @@ def test_a_replayed_step_takes_the_drafts_away(dev):
     m.forward_tree([[1, 2]], [[-1, 0]], [3])
     m.verify_tree()
     m.free()
+
+
+def test_a_pass_that_fails_leaves_none_to_judge(dev):
+    """Where one of a pass's calls is refused, neither its half-made states nor
+    an earlier pass's, whose draft entries it has begun to replace, are there."""
+    m = _drafted(dev)
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    m.verify_tree()
+    call = m._call
+
+    def refuse(name, *args):
+        if name == "gx_qwen_attention_tree":
+            raise MemoryError(name)
+        call(name, *args)
+
+    m._call = refuse
+    with pytest.raises(MemoryError):
+        m.forward_tree([[7, 8]], [[-1, 0]], [3])
+    m._call = call
+    for step in (m.verify_tree, m.commit_tree):
+        with pytest.raises(ValueError, match="no pass over drafted"):
+            step()
+    # a pass refused for its arguments has replaced nothing
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+    want = [x.clone() for x in m.verify_tree()]
+    with pytest.raises(ValueError, match="no earlier node"):
+        m.forward_tree([[7, 8]], [[-1, 4]], [3])
+    for x, y in zip(want, m.verify_tree()):
+        assert torch.equal(x, y)
+    m.commit_tree()
+    m.free()
