@@ -717,9 +717,9 @@ class QwenModel:
         if uniforms is None and temperature > 0:
             uniforms = torch.rand((M,), device="cuda")
         for x, shape, what in ((draft_logits, (M, V), "draft logits"), (uniforms, (M,), "random numbers")):
-            if x is not None and not (tuple(x.shape) == shape and x.dtype == torch.float32 and x.is_cuda
-                                      and x.is_contiguous()):
-                raise ValueError(f"qwen: the {what} are a contiguous float32 {shape} on the GPU, not "
+            if x is not None and not (tuple(x.shape) == shape and x.dtype == torch.float32
+                                      and x.device == self.tokens.device and x.is_contiguous()):
+                raise ValueError(f"qwen: the {what} are a contiguous float32 {shape} on {self.tokens.device}, not "
                                  f"{x.dtype} {tuple(x.shape)} on {x.device}")
         logits = self.logits_batch(range(M))
         ws, size = self._tree_workspace("gx_tree_verify_workspace_bytes", t["n"], M, V)

@@ -85,3 +85,27 @@ def test_a_pass_that_fails_leaves_none_to_judge(dev):
         assert torch.equal(x, y)
     m.commit_tree()
     m.free()
+
+
+def test_tensors_of_another_gpu_are_refused(dev):
+    """Random numbers and draft logits that are not on the model's device."""
+    m = _drafted(dev)
+    m.forward_tree([[1, 2]], [[-1, 0]], [3])
+
+    class Elsewhere:
+        dtype, is_cuda, device = torch.float32, True, torch.device("cuda", 1)
+
+        def __init__(self, *shape):
+            self.shape = shape
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            raise AssertionError("its address was asked for")
+
+    with pytest.raises(ValueError, match="random numbers.*cuda:1"):
+        m.verify_tree(0.5, uniforms=Elsewhere(2))
+    with pytest.raises(ValueError, match="draft logits.*cuda:1"):
+        m.verify_tree(0.5, draft_logits=Elsewhere(2, m.cfg.vocab), uniforms=torch.rand(2, device="cuda"))
+    m.free()
