@@ -230,18 +230,16 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
             int p0, lo, hi;
             const bool draft = rows_of(j, p0, lo, hi);
             // Keys and chunks of values past the rows that there are repeat one that is
-            // (its chance will be zero); the rows beside those in a chunk become zero.
-            const int cl = p0 < lo ? (lo - p0) >> 3 : -1, ch = p0 + kStage > hi ? (hi - p0) >> 3 : -1;
-            if ((cl >= 0 && (lo & 7)) || (ch >= 0 && (hi & 7))) {
-                for (int e = tid; e < HD; e += 64 * nw) {
-                    uint8_t *vr = st + HD * 128 + e * 128;
-                    if (cl >= 0) {
-                        v8h *to = (v8h *)(vr + ((cl ^ (e & 7)) << 4));
-                        *to = keep(*to, lo - (p0 + 8 * cl), hi - (p0 + 8 * cl));
-                    }
-                    if (ch >= 0 && ch < 8) {
-                        v8h *to = (v8h *)(vr + ((ch ^ (e & 7)) << 4));
-                        *to = keep(*to, lo - (p0 + 8 * ch), hi - (p0 + 8 * ch));
+            // (its chance will be zero).  The rows beside those become zero, in the
+            // chunk with the first and in the chunk with the last and every copy of it:
+            // a NaN there would make 0 * NaN in every row's sums.
+            const int cl = p0 < lo ? 0 : 8, ch = p0 + kStage > hi && (hi & 7) ? (hi - p0) >> 3 : 8;
+            if (cl < 8 || ch < 8) {
+                for (int i = tid; i < 8 * HD; i += 64 * nw) {
+                    const int e = i >> 3, c = i & 7;
+                    if (c == cl || c >= ch) {
+                        v8h *to = (v8h *)(st + HD * 128 + e * 128 + ((c ^ (e & 7)) << 4));
+                        *to = keep(*to, lo - (p0 + 8 * c), hi - (p0 + 8 * c));
                     }
                 }
                 lds_barrier();
