@@ -1,11 +1,14 @@
 """The attention of drafted trees where a workgroup takes several steps of keys
-in a row, and what lies behind a tree's rows."""
+in a row: whole ones and partial ones, prefix and drafts, maxima that rise from
+one to the next; what lies behind a tree's rows; and the precision that the
+probabilities' second part gives."""
 import math
 
 import numpy as np
 import pytest
 
 from golem_amd import capi, synth
+from tests.gpu_util import log
 from tests.test_gpu_tree import Attention, long_context, offsets
 
 gpu = pytest.mark.gpu
@@ -88,6 +91,28 @@ def many(name, seed, **kw):
     return a
 
 
+@gpu
+@pytest.mark.parametrize("ramp", [0.0, 14.0, 120.0, -120.0])
+@pytest.mark.parametrize("name", MANY)
+def test_many_steps_a_share(dev, name, ramp):
+    """Whole and partial steps of the prefix and the drafts in one share; with a
+    ramp the maximum rises past the reference at some steps, or at every one, or
+    is the first one's."""
+    many(name, 300, ramp=ramp, pad=3).behind(0.25).check(dev)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["three", "five", "eight"])
+@pytest.mark.parametrize("prefix", [576, 577, 583, 584, 607, 608, 609, 639, 640])
+def test_many_steps_and_prefixes(dev, name, prefix):
+    """The prefix's last step of every kind: whole, one key, and ends on and off a
+    chunk of eight and a half of the step."""
+    heads, kv, hd, sizes, _, trees, _ = MANY[name]
+    a = Steps(301, [sizes[0] - 1, 11], [prefix, prefix - 5], heads, kv, hd, trees=2 * trees, most=1600)
+    assert a.launch()[0] and a.launch()[1] >= 3, a.launch()
+    a.check(dev)
+
+
 def bits(x):
     return np.ascontiguousarray(x).view(np.uint32)
 
@@ -122,3 +147,60 @@ def test_another_trees_rows_leave_no_trace(dev, name):
     for value in (np.inf, np.nan):
         a.kd[:, t:], a.vd[:, t:] = value, value
         np.testing.assert_array_equal(bits(a.run(dev)[:t]), bits(want[:t]))
+
+
+# ---- the probabilities' precision ---------------------------------------------------
+
+
+def value_bound(count):
+    """How far o / v may be from 1 where every key has the value v.  The scores'
+    errors are in numerator and denominator alike and cancel.  A probability's
+    two parts, each cut off after eleven bits, are it but for less than 2^-21 of
+    it, or 2^-24 where the second is below fp16's normal numbers; the row's sum is
+    2^8 at least.  Every float32 addition is off by half a step, 2^-24, of a sum
+    that is never above the last: one a term in the denominator and two (a part
+    each) in the numerator, and 64 more each for rescalings, wavefronts and
+    shares; four for the weights' products, the quotient and the output."""
+    return 3 * (count + 64) * 2.0 ** -24 + 2.0 ** -21 + count * 2.0 ** -32 + 4 * 2.0 ** -24
+
+
+def cut(p, least):
+    """p with its leading eleven bits, or down to `least`."""
+    e = np.floor(np.log2(np.maximum(p, 1e-300)))
+    step = np.maximum(2.0 ** (e - 10), least)
+    return np.floor(p / step) * step
+
+
+@pytest.mark.parametrize("count", [300, 520, 720])
+def test_the_bound_tells_one_part_from_two(count):
+    """The bound below holds for two parts and for one part does not (the sums
+    exact here: their roundings are what the bound has besides)."""
+    g = synth.rng(310)
+    for _ in range(20):
+        p = 256.0 * np.exp2(np.minimum(g.standard_normal(count) * 0.7 - 2, 0)).astype(np.float32).astype(np.float64)
+        p[0] = 256.0
+        one = cut(p, 2.0 ** -24)
+        two = one + cut(p - one, 2.0 ** -24)
+        assert abs(two.sum() / p.sum() - 1) < 2.0 ** -21 + count * 2.0 ** -32
+        assert abs(one.sum() / p.sum() - 1) > 1.5 * value_bound(count)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv,hd,sizes,prefix,trees,most", [
+    (4, 2, 64, [9], [300], 1, 0), (8, 2, 128, [6, 4], [511, 300], 2, 0), (4, 2, 64, [40], [520], 1, long_context(1, 40, 4, 2)),
+    MANY["three"], MANY["five"], MANY["nine"], MANY["two"]])
+def test_values_all_alike_come_back(dev, heads, kv, hd, sizes, prefix, trees, most):
+    """Every key of a head with one value an element: that value is the result.  A
+    probability that lost its second part on the way to the values would leave
+    3.5e-4 of it behind."""
+    a = Steps(311, sizes, prefix, heads, kv, hd, trees=trees, most=most, spread=0.5)
+    v = (1.0 + np.arange(kv * hd).reshape(kv, 1, hd) % 61 / 64).astype(np.float16)
+    a.v[:], a.vd[:] = v, v
+    got = a.run(dev)[:a.tokens].astype(np.float64).reshape(a.tokens, kv, heads // kv, hd)
+    off = np.abs(got / v.astype(np.float64).reshape(kv, 1, hd) - 1)
+    worst = 0.0
+    for b, t in enumerate(sizes):
+        rows = slice(a.first[b], a.first[b] + t)
+        worst = max(worst, off[rows].max() / value_bound(prefix[b] + t))
+    log(f"  worst {off.max():.2e}, {worst:.3f} of the bound")
+    assert worst <= 1
