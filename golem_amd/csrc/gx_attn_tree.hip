@@ -16,9 +16,10 @@
 // never leave the registers.
 //
 // A probability enters the second product as two fp16 values, its leading 11
-// bits and the rest (about 22 bits together): rounded to one, the head
-// outputs would be 2e-4 off, which the float output could not hide.  Sums,
-// maxima and outputs are float32.
+// bits and the next 11, cut off: together within 2^-21 of it, or within 2^-32 of
+// the row's largest where that is more (the second then below fp16's normal
+// numbers).  The leading bits alone would leave a head's outputs 3.5e-4 short,
+// which the float output could not hide.  Sums, maxima and outputs are float32.
 //
 // Two kernels and a join of the keys' shares.  Trees of one tile of rows (eight
 // nodes of four query heads a key-value head, say) move bytes more than they
@@ -136,18 +137,26 @@ __device__ __forceinline__ void chances(const v16f &s, int w, float c, float bas
 // group: key-value heads fastest, so that with eight of them every workgroup
 // of a head is on one XCD and shares its L2.
 //
-// Bound by the matrix instructions: 64 nodes of 32 heads over 8, 128 wide, and
-// 32000 positions take 60 us (48 a step and wavefront at 30 ns each, where a
-// large fp16 product of a library reaches 28), 2.2 TB/s of keys and values; the
-// join 8 us.  A second wavefront a SIMD adds nothing then, nor did scores and
-// products of neighbouring steps side by side (65 us), a longer ring, or an
-// order of the instructions laid down by hand.
+// 64 nodes of 32 heads over 8, 128 wide, and 32000 positions take 60 us, 2.2
+// TB/s of keys and values; the join 8 us.  Some 45 of the 60 are matrix
+// instructions: 1500 a SIMD (48 a step and wavefront) at 30 ns each, where a
+// large fp16 product of a library reaches 28; they keep the matrix units busy
+// for 47 % of the kernel's cycles by the counters.  What is left was not taken
+// apart: the launch, the first step's loads, and the shares' outputs, 34 MB
+// that all workgroups write at the end.  A second wavefront a SIMD adds nothing
+// to a step's rate, nor did scores and products of neighbouring steps side by
+// side (65 us), a longer ring, or an order of the instructions laid down by
+// hand.  Eight trees of up to 33 nodes over 1500 positions take 23.5 us: 15 of
+// matrix instructions on the SIMDs that have one and a half tiles of a 33-node
+// tree (every tree gets the same shares, so that the average SIMD has half of
+// that).
 //
 // A step's 64 keys and values come into LDS by direct loads, one step ahead of
 // the products, for every tile of the group: the keys as 1 KiB pieces of 64
 // positions, a value row's 128 bytes with its eight 16-byte chunks exchanged
 // by the row's low bits, so that both the loads (eight whole rows each) and
-// the operand reads (a chunk of 32 rows) are without conflicts.
+// the operand reads (a chunk of 32 rows) go round the banks (two cycles of
+// conflict an LDS instruction by the counters).
 template <int HD>
 __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x) {
     constexpr int KS = HD / 16, ET = HD / 32, kSlot = HD * 256;
@@ -157,7 +166,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void attn_tree_kernel(const Args x)
     const int kvh = blockIdx.x, b = blockIdx.z / x.S, sp = blockIdx.z % x.S;
     const Tree t(x, b, kStage);
     // Five or six tiles: the first four a wavefront each, the others two, one of
-    // each step's halves each, so that no SIMD has two whole tiles (eight trees of
+    // a step's halves each, so that no SIMD has two whole tiles (eight trees of
     // 33 nodes over 4000 positions 46 us, and 51 with five whole ones; of 80, 81 and 91).
     const int tiles = x.halves ? nw / 2 + 2 : nw, whole = x.halves ? 4 : nw;
     const int half = wave < whole ? 0 : (wave - whole) & 1, tile = wave < whole ? wave : whole + (wave - whole) / 2;

@@ -39,8 +39,11 @@ __global__ __launch_bounds__(256) void cache_commit_kernel(const CommitLayers at
     // of the keys), whose bytes lie together on both sides; all of a thread's
     // loads before its stores, the values' past the caches (kept there, sixteen
     // paths of twelve through 36 layers take 45 us where this takes 37; the keys'
-    // past them too 42).  Bound by the stores' pieces: 24 bytes of values and 192
-    // of keys lie together, 69 MB move where 44 are wanted.  (An element's
+    // past them too 42).  Of the 37 us the bytes are 15 at a large copy's rate (30
+    // MB read and 42 written by the counters where 22 each are wanted: 24 bytes of
+    // values and 192 of keys lie together), and the vector instructions, most of
+    // them index arithmetic, 11 (5900 a SIMD); the wavefronts spend 44 % of their
+    // time waiting for memory and 49 % for their turn to issue.  (An element's
     // positions a thread: each store on a line of its own, 74 us; two positions a
     // word a thread: 46.)
     v4u_stream *kc = (v4u_stream *)(at.kc[layer] + to);

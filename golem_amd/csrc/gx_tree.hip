@@ -513,7 +513,7 @@ constexpr int kLooks = 16;   // looks of the walk for workgroups that have not j
 // grid (groups, n): a tree's first workgroup walks, the others help.
 //
 // Bound by round trips to memory shared among the XCDs.  Eight chains of up to six
-// nodes over 151936 tokens take 18 us, four trees of up to 33 take 37: some 10 us to
+// nodes over 151936 tokens take 18 us, four trees of up to 33 take 35 to 38: some 10 us to
 // begin (the tree, its rows' sums, the children's chances, the others joining),
 // about 4 a sum, two loads and a scan to draw the last token.  A workgroup a tree
 // alone takes 360 and 590; parts handed out by a claim of each workgroup 20

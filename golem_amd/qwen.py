@@ -112,7 +112,8 @@ class QwenModel:
     the matrix cores: golem's values within float rounding, so a prompt read
     in one batch and the same tokens read one at a time agree only to that
     rounding.  "golem" keeps golem's serial order bit for bit, and with it
-    golem's batch == one at a time."""
+    golem's batch == one at a time.  Trees of drafted tokens (forward_tree) run
+    in one order under both, another than either's."""
 
     def __init__(self, ctx, cfg, weights, max_batch, attention="parallel"):
         if attention not in ("parallel", "golem"):
@@ -622,7 +623,14 @@ class QwenModel:
         conversation slots[b] (default: the current slot, for one tree) has
         cached.  Returns the device hidden states [M][dim] after the final
         norm, the trees' nodes one after another; the caches stay as they are
-        until commit_tree."""
+        until commit_tree.  The attention's sums are in an order of their own:
+        a node's state is what its path run alone gives but for float rounding
+        (and what that moves in the Q8_0 activations after it).  A token outside
+        the vocabulary may be among the drafts (verify_tree passes it over),
+        but its NaN entries make every layer's attention sum the rest of its
+        tree again key by key, many times the pass without it.  As any pass
+        does, this one replaces the device's tokens and positions: seed a
+        lock-step or captured decode again after it."""
         n, sizes = len(tokens), [len(t) for t in tokens]
         slots = [self.slot] * n if slots is None else list(slots)
         M, nodes = sum(sizes), max(sizes, default=0)
@@ -705,8 +713,10 @@ class QwenModel:
         decoding would have drawn; above, each node's number in `uniforms`
         (device float32 [M], in [0, 1); default: torch's generator) decides,
         the drafts being given tokens or, with draft_logits (device [M][vocab],
-        the draft model's logits after each node), drawn from their softmax at
-        draft_temperature (default: temperature).  No other pass may have run
+        the draft model's logits after each node), drawn from the softmax of
+        their parent's row at draft_temperature (default: temperature),
+        siblings without replacement in their order: only then are the tokens
+        distributed as the target's own.  No other pass may have run
         since: the model's own are noticed and refused, replays of a graph that
         a caller captured over them are not.  Returns device tensors:
         path [trees][nodes] (-1 behind), counts [trees], next [trees]."""
@@ -760,9 +770,13 @@ class QwenModel:
         kept.  draft(ids) proposes a tree after the ids so far: (tokens,
         parents) of nodes 1, 2, .., parents as node numbers with 0 the last
         id, or with a third entry (or None), the device draft logits
-        [1 + nodes][vocab] that the tokens were drawn from.  temperature 0: greedy's tokens;
-        above, random numbers come from `generator` (a torch generator of the
-        GPU).  Returns the ids and the number of passes."""
+        [1 + nodes][vocab] that the tokens were drawn from: each node's from its
+        parent's row at `temperature`, siblings without replacement
+        (verify_tree).  temperature 0: the target's best tokens, which are
+        greedy()'s unless two logits are closer than the orders of the
+        attention's sums move them (forward_tree); above, random numbers come
+        from `generator` (a torch generator of the GPU).  Returns the ids and
+        the number of passes."""
         if not prompt or len(prompt) + steps - 1 > self.slot_context:
             raise ValueError(f"qwen: {steps} tokens after {len(prompt)} exceed the context {self.slot_context}")
         if self.drafts == 0:
