@@ -189,7 +189,7 @@ class QwenModel:
         self.tree_ws, self.tree_ws_kept = None, []
         self.pool = None  # pages (set_pages)
         self.page_batch, self.page_graphs = None, {}  # the conversations in lock step, their captured steps
-        self.page_ws, self.page_ws_kept = None, []
+        self.page_ws = None
         self.tree_states = False  # the tokens and hidden states are forward_tree's
         n = capi.size_out("gx_qwen_attention_workspace_bytes", M, cfg.heads, cfg.max_context - 1)
         self.attn_ws = torch.empty((n + 255) // 256 * 256, dtype=torch.uint8, device="cuda")
@@ -868,7 +868,8 @@ class QwenModel:
             raise ValueError(f"qwen: pages hold heads of 32, 64, 96 and 128, not {cfg.head_dim}")
         shape = (count, cfg.kv_heads, size, cfg.head_dim)
         dtype = torch.int16 if kind == "fp16" else torch.int8
-        self.pool = None
+        # (what works on the last one first: a captured step holds its addresses)
+        self.pool, self.page_batch, self.page_graphs, self.page_ws = None, None, {}, None
         self.pool = {
             "count": count, "size": size, "kind": capi.PAGES_F16 if kind == "fp16" else capi.PAGES_I8,
             "k": [torch.zeros(shape, dtype=dtype, device=dev) for _ in range(cfg.layers)],
@@ -878,7 +879,6 @@ class QwenModel:
             "free": list(range(count - 1, -1, -1)), "held": [0] * count,  # pages, and how many conversations hold each
             "lists": {}, "lengths": {}, "next": 0,                        # conversations' pages and positions
         }
-        self.page_batch, self.page_graphs = None, {}
 
     def _a_pool(self):
         if self.pool is None:
@@ -960,11 +960,16 @@ class QwenModel:
              vp(self.set8.qs), vp(self.page_ws), self.page_ws.numel())
 
     def _page_workspace(self, t):
+        """A workspace for t's attention: the passes share one, which goes back to
+        the allocator when a larger one takes its place (in stream order, as the
+        pass's other tensors do), but for captured steps that hold it.  It at least
+        doubles, so that what those hold is less than the one in use."""
         n = max(256, (capi.size_out("gx_qwen_attention_paged_workspace_bytes", t["n"], t["M"], t["tokens"], self.cfg.heads,
                                     self.cfg.kv_heads, self.cfg.head_dim, t["bound"]) + 255) // 256 * 256)
         if self.page_ws is None or self.page_ws.numel() < n:
-            self.page_ws_kept.append(self.page_ws)  # a captured step may hold its address
-            self.page_ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+            last = 0 if self.page_ws is None else self.page_ws.numel()
+            self.page_ws = None
+            self.page_ws = torch.empty(max(n, 2 * last), dtype=torch.uint8, device="cuda")
 
     def forward_pages(self, tokens, conversations):
         """One pass over new tokens of several conversations in the pages:
@@ -1049,6 +1054,7 @@ class QwenModel:
         self._page_workspace(t)
         if graph and t["graph"] is None:
             t["graph"] = self._capture(lambda: self._pages_device_step(t))
+            t["ws"] = self.page_ws  # whose address the graph holds
         if graph:
             t["graph"].replay()
         else:

@@ -271,3 +271,58 @@ def test_rope_scaling(dev):
     np.testing.assert_array_equal(bits(m.rope_cos), tables[0])
     np.testing.assert_array_equal(bits(m.forward(p, 0)), plain)
     m.free()
+
+
+def test_workspaces_of_passes_over_pages_go_back(dev):
+    """Passes of rising sizes leave no more behind than a few times the largest
+    one's workspace, and a new pool leaves none."""
+    cfg = synth.QwenConfig(256, 512, 2, 16, 1, 64, 1024, 2048)
+    m = model(dev, 110, cfg, 400)
+    m.set_pages(64, 64)
+    m.forward_pages([prompt(111, 8)], [m.open_conversation()])
+    before, largest = torch.cuda.memory_allocated(), 0
+    for k in range(40, 400, 8):
+        c = m.open_conversation()
+        for piece in range(3):
+            m.forward_pages([prompt(112 + piece, k)], [c])
+            largest = max(largest, capi.size_out("gx_qwen_attention_paged_workspace_bytes", 1, k, k, 16, 1, 64, (piece + 1) * k))
+        m.close_conversation(c)
+    log(f"  {torch.cuda.memory_allocated() - before} bytes more, the largest workspace {largest}")
+    assert largest > 4 << 20 and torch.cuda.memory_allocated() - before <= 4 * largest
+    m.set_pages(1, 16)
+    m.pool = None
+    assert torch.cuda.memory_allocated() < before
+    m.free()
+
+
+def test_captured_steps_keep_their_workspace(dev):
+    """A captured step replayed after a pass whose workspace outgrew its own, and
+    after what that freed has been written over, gives the eager step's bits."""
+    cfg = synth.QwenConfig(256, 512, 2, 16, 1, 64, 1024, 4096)
+    runs = []
+    for graph in (False, True):
+        m = model(dev, 113, cfg, 400)
+        m.set_pages(128, 64)
+        c = m.open_conversation()
+        for piece in range(6):
+            m.forward_pages([prompt(114 + piece, 400)], [c])
+        m.page_ws = None  # (the captured step's own is then a small one)
+        m.start_pages([3], [c])
+        seen = []
+        for step in range(6):
+            ids = m.pages_step(graph).cpu().numpy().copy()
+            seen.append((ids, bits(m.hidden[:1]), bits(m.logit[:1])))
+            if step in (1, 3):
+                other = m.open_conversation()
+                for piece in range(3):
+                    m.forward_pages([prompt(5 + piece, 390)], [other])
+                m.close_conversation(other)
+                held = [torch.full((1 << k,), 0xFF, dtype=torch.uint8, device="cuda") for k in range(12, 26) for _ in range(3)]
+                torch.cuda.synchronize()
+                del held
+                m.start_pages(torch.from_numpy(ids).cuda(), [c])
+        runs.append(seen)
+        m.free()
+    for x, y in zip(*runs):
+        for a, b in zip(x, y):
+            np.testing.assert_array_equal(a, b)
