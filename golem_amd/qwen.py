@@ -52,6 +52,7 @@ a batch in lock step: the blocks with gx_qwen_qk_rope_paged and
 gx_qwen_attention_paged.  set_rope_scaling stretches the rotations of every
 kind of pass to longer contexts (gx_rope_tables).
 """
+import contextlib
 import ctypes
 import math
 import weakref
@@ -926,8 +927,10 @@ class QwenModel:
     def conversation_length(self, c):
         return self._a_conversation(c)["lengths"][c]
 
-    def _grow(self, wanted):
-        """Pages for conversations c to hold wanted[c] positions: all, or none and an error."""
+    @contextlib.contextmanager
+    def _grown(self, wanted):
+        """A pass for which conversations c hold pages for wanted[c] positions: all
+        of them, or none and an error.  Those taken for a pass that fails go back."""
         p = self.pool
         need = {c: (w + p["size"] - 1) // p["size"] - len(p["lists"][c]) for c, w in wanted.items()}
         if sum(max(x, 0) for x in need.values()) > len(p["free"]):
@@ -937,6 +940,15 @@ class QwenModel:
                 page = p["free"].pop()
                 p["held"][page] = 1
                 p["lists"][c].append(page)
+        try:
+            yield
+        except BaseException:
+            for c, x in reversed(need.items()):
+                for _ in range(x):
+                    page = p["lists"][c].pop()
+                    p["held"][page] = 0
+                    p["free"].append(page)
+            raise
 
     def _page_lists(self, conversations, width):
         table = np.full((len(conversations), width), -1, np.int32)
@@ -991,7 +1003,15 @@ class QwenModel:
             lengths[c] = self._a_conversation(c)["lengths"][c] + x
             if lengths[c] > self.cfg.max_context:
                 raise ValueError(f"qwen: {lengths[c]} positions exceed the context {self.cfg.max_context}")
-        self._grow(lengths)
+        with self._grown(lengths):
+            self._pages_pass(tokens, conversations, sizes, lengths)
+        for c in conversations:
+            p["lengths"][c] = lengths[c]
+        return self.hidden[:M]
+
+    def _pages_pass(self, tokens, conversations, sizes, lengths):
+        """forward_pages once the conversations hold the pages for lengths[c] positions."""
+        p, n, M = self.pool, len(tokens), sum(sizes)
 
         def dev(v):
             return torch.tensor(np.asarray(v, dtype=np.int32), device="cuda")
@@ -1001,13 +1021,12 @@ class QwenModel:
              "bound": max(lengths.values()),
              "table": self._page_lists(conversations, max(len(p["lists"][c]) for c in conversations)).cuda()}
         self._page_workspace(t)
-        self.tokens[:M].copy_(dev([y for x in tokens for y in x]))
-        self.positions[:M].copy_(dev(np.concatenate([np.arange(lengths[c] - x, lengths[c])
-                                                     for c, x in zip(conversations, sizes)])))
+        ids = dev([y for x in tokens for y in x])
+        at = dev(np.concatenate([np.arange(lengths[c] - x, lengths[c]) for c, x in zip(conversations, sizes)]))
+        self.tree_states, self.page_batch = False, None  # their tokens are replaced
+        self.tokens[:M].copy_(ids)
+        self.positions[:M].copy_(at)
         self._blocks(M, 0, attend=lambda i: self._attend_pages(i, t))
-        for c in conversations:
-            p["lengths"][c] = lengths[c]
-        return self.hidden[:M]
 
     def start_pages(self, tokens, conversations):
         """Seeds lock-step decoding of conversations in the pages: token i (a
@@ -1040,8 +1059,17 @@ class QwenModel:
         n, top = len(batch), 1 + max(p["lengths"][c] for c in batch)
         if top > cfg.max_context:
             raise ValueError(f"qwen: {top} positions exceed the context {cfg.max_context}")
-        self._grow({c: p["lengths"][c] + 1 for c in batch})
-        bound = min(cfg.max_context, max(256, 1 << (top - 1).bit_length()))
+        with self._grown({c: p["lengths"][c] + 1 for c in batch}):
+            self._pages_one_step(n, min(cfg.max_context, max(256, 1 << (top - 1).bit_length())), graph)
+        for c in batch:
+            p["lengths"][c] += 1
+        self.page_batch = batch
+        return self.next_id[:n]
+
+    def _pages_one_step(self, n, bound, graph):
+        """pages_step once the conversations hold the pages for one position more, for
+        lengths of at most `bound`."""
+        p, batch = self.pool, self.page_batch
         if (n, bound) not in self.page_graphs:
             width = (bound + p["size"] - 1) // p["size"]
             t = {"n": n, "M": n, "tokens": 1, "bound": bound, "first": torch.arange(n + 1, dtype=torch.int32, device="cuda"),
@@ -1059,10 +1087,6 @@ class QwenModel:
             t["graph"].replay()
         else:
             self._pages_device_step(t)
-        for c in batch:
-            p["lengths"][c] += 1
-        self.page_batch = batch
-        return self.next_id[:n]
 
     def _pages_device_step(self, t):
         n = t["n"]

@@ -326,3 +326,45 @@ def test_captured_steps_keep_their_workspace(dev):
     for x, y in zip(*runs):
         for a, b in zip(x, y):
             np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("where", ["tokens", "workspace", "blocks"])
+def test_a_pass_that_fails_takes_no_pages(dev, where):
+    """Pages, lengths and later steps as if the failed pass had not been asked for."""
+    cfg = synth.QwenConfig(256, 512, 2, 4, 2, 64, 1024, 1024)
+    m = model(dev, 115, cfg, 400)
+    m.set_pages(60, 16)
+    c, d = m.open_conversation(), m.open_conversation()
+    m.forward_pages([prompt(116, 20), prompt(117, 9)], [c, d])
+    free, lists = list(m.pool["free"]), {k: list(v) for k, v in m.pool["lists"].items()}
+
+    def fail(*a, **kw):
+        raise RuntimeError("out of memory")
+
+    if where == "tokens":
+        with pytest.raises((TypeError, ValueError)):
+            m.forward_pages([["x"] * 350, [1]], [c, d])
+    else:
+        name = {"workspace": "_page_workspace", "blocks": "_blocks"}[where]
+        setattr(m, name, fail)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            m.forward_pages([prompt(118, 350), [1]], [c, d])
+        m.start_pages([1, 2], [c, d])
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="out of memory"):
+                m.pages_step()
+        delattr(m, name)
+    assert m.pool["free"] == free and m.pool["lists"] == lists
+    assert m.pool["held"] == [sum(p in x for x in lists.values()) for p in range(60)]
+    assert m.conversation_length(c) == 20 and m.conversation_length(d) == 9
+    other = model(dev, 115, cfg, 400)
+    other.set_pages(60, 16)
+    cs = [other.open_conversation() for _ in range(2)]
+    other.forward_pages([prompt(116, 20), prompt(117, 9)], cs)
+    for x, y in ((m, [c, d]), (other, cs)):
+        x.start_pages([1, 2], y)
+    for _ in range(14):
+        np.testing.assert_array_equal(m.pages_step().cpu().numpy(), other.pages_step().cpu().numpy())
+        np.testing.assert_array_equal(bits(m.hidden[:2]), bits(other.hidden[:2]))
+    other.free()
+    m.free()
