@@ -188,7 +188,7 @@ class QwenModel:
         self.slot_graphs = {}
         self.drafts = 0  # tokens the draft buffers hold (set_drafts)
         self.tree_ws, self.tree_ws_kept = None, []
-        self.pool = None  # pages (set_pages)
+        self.pool, self.conversations = None, 0  # pages (set_pages), and the conversations opened in any so far
         self.page_batch, self.page_graphs = None, {}  # the conversations in lock step, their captured steps
         self.page_ws = None
         self.tree_states = False  # the tokens and hidden states are forward_tree's
@@ -858,8 +858,9 @@ class QwenModel:
     def set_pages(self, count, size=64, kind="fp16"):
         """A pool of `count` pages of `size` positions (a power of two from 16
         to 1024) a layer, for conversations beside the slots'; replaces the
-        last pool and its conversations.  kind: "fp16", or "int8" with a scale
-        for each head and position, in half the bytes."""
+        last pool and its conversations, whose numbers are not given out again.
+        kind: "fp16", or "int8" with a scale for each head and position, in
+        half the bytes."""
         cfg, dev = self.cfg, "cuda"
         if count < 1 or size < 16 or size > 1024 or size & (size - 1):
             raise ValueError(f"qwen: {count} pages of {size} positions (a power of two from 16 to 1024)")
@@ -878,7 +879,7 @@ class QwenModel:
             "ks": [torch.zeros(shape[:3], device=dev) if kind == "int8" else None for _ in range(cfg.layers)],
             "vs": [torch.zeros(shape[:3], device=dev) if kind == "int8" else None for _ in range(cfg.layers)],
             "free": list(range(count - 1, -1, -1)), "held": [0] * count,  # pages, and how many conversations hold each
-            "lists": {}, "lengths": {}, "next": 0,                        # conversations' pages and positions
+            "lists": {}, "lengths": {},                                   # conversations' pages and positions
         }
 
     def _a_pool(self):
@@ -895,8 +896,8 @@ class QwenModel:
     def open_conversation(self):
         """A conversation of no positions in the pages; its number."""
         p = self._a_pool()
-        c = p["next"]
-        p["next"] += 1
+        c = self.conversations
+        self.conversations += 1
         p["lists"][c], p["lengths"][c] = [], 0
         return c
 

@@ -368,3 +368,18 @@ def test_a_pass_that_fails_takes_no_pages(dev, where):
         np.testing.assert_array_equal(bits(m.hidden[:2]), bits(other.hidden[:2]))
     other.free()
     m.free()
+
+
+def test_conversations_of_a_replaced_pool_are_gone(dev):
+    """A number from before set_pages names no conversation of the new pool."""
+    m = model(dev)
+    m.set_pages(4, 16)
+    old = m.open_conversation()
+    m.set_pages(4, 16)
+    new = m.open_conversation()
+    assert new != old
+    for call in (lambda: m.forward_pages([[1]], [old]), lambda: m.start_pages([1], [old]),
+                 lambda: m.share_conversation(old, 0), lambda: m.close_conversation(old)):
+        with pytest.raises(IndexError, match=f"no conversation {old} "):
+            call()
+    m.free()
