@@ -187,10 +187,11 @@ def last_error():
 
 class Context:
     """One gx_ctx on a device.  stream: a hipStream_t as an int, or None for
-    the null stream."""
+    the null stream; a model's captures leave the context on it."""
 
     def __init__(self, device=0, stream=None):
         self.ptr = ctypes.c_void_p()
+        self.stream = stream
         call("gx_init", device, ctypes.byref(self.ptr))
         if stream is not None:
             call("gx_set_stream", self.ptr, ctypes.c_void_p(stream))

@@ -423,25 +423,28 @@ class QwenModel:
         self._call("gx_argmax_step", self.ctx.ptr, self._vp(self.logit), self.cfg.vocab, self._vp(self.tokens),
                    self._vp(self.history), self.history.numel(), self._vp(self.pos_dev), self._vp(self.positions))
 
-    def capture_decode(self):
-        """Records _decode_step into a HIP graph (once).  The library's stream
-        is the capture stream while recording."""
-        if self.graph is not None:
-            return
-        if self.nslots > 1:
-            raise ValueError("qwen: the captured decode step serves one conversation")
+    def _capture(self, step):
+        """step recorded into a graph.  The library's stream is the capture stream
+        while recording, and then the context's own again."""
         torch.cuda.synchronize()
-        stream = torch.cuda.Stream()
-        graph = _Step()
+        stream, graph = torch.cuda.Stream(), _Step()
         graph.model = weakref.proxy(self)
         self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(stream.cuda_stream))
         try:
             with torch.cuda.graph(graph, stream=stream):
-                self._decode_step()
+                step()
         finally:
-            self._call("gx_set_stream", self.ctx.ptr, None)
+            self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(self.ctx.stream))
         torch.cuda.synchronize()
-        self.graph = graph
+        return graph
+
+    def capture_decode(self):
+        """Records _decode_step into a HIP graph (once)."""
+        if self.graph is not None:
+            return
+        if self.nslots > 1:
+            raise ValueError("qwen: the captured decode step serves one conversation")
+        self.graph = self._capture(self._decode_step)
 
     def logits(self, row):
         """Logits of hidden state `row` (of the last forward): the tied head
@@ -512,18 +515,7 @@ class QwenModel:
             return
         if not 0 < n <= min(self.nslots, self.max_batch):
             raise ValueError(f"qwen: {n} conversations for {self.nslots} slots")
-        torch.cuda.synchronize()
-        stream = torch.cuda.Stream()
-        graph = _Step()
-        graph.model = weakref.proxy(self)
-        self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(stream.cuda_stream))
-        try:
-            with torch.cuda.graph(graph, stream=stream):
-                self._slots_device_step(n, self.slot_context - 1)
-        finally:
-            self._call("gx_set_stream", self.ctx.ptr, None)
-        torch.cuda.synchronize()
-        self.slot_graphs[n] = graph
+        self.slot_graphs[n] = self._capture(lambda: self._slots_device_step(n, self.slot_context - 1))
 
     def logits_batch(self, rows):
         """LogitsBatch (qwen/model.go:200-214): the logits of several hidden
@@ -1096,20 +1088,6 @@ class QwenModel:
         self.logits_batch(range(n))
         self._call("gx_argmax_slots_step", self.ctx.ptr, self._vp(self.logit), self.cfg.vocab, n, self.cfg.vocab,
                    self._vp(self.next_id), self._vp(self.tokens), self._vp(self.positions))
-
-    def _capture(self, step):
-        """step recorded into a graph, the library's stream being the capture's."""
-        torch.cuda.synchronize()
-        stream, graph = torch.cuda.Stream(), _Step()
-        graph.model = weakref.proxy(self)
-        self._call("gx_set_stream", self.ctx.ptr, ctypes.c_void_p(stream.cuda_stream))
-        try:
-            with torch.cuda.graph(graph, stream=stream):
-                step()
-        finally:
-            self._call("gx_set_stream", self.ctx.ptr, None)
-        torch.cuda.synchronize()
-        return graph
 
     def free(self):
         for b in self.blocks:

@@ -383,3 +383,33 @@ def test_conversations_of_a_replaced_pool_are_gone(dev):
         with pytest.raises(IndexError, match=f"no conversation {old} "):
             call()
     m.free()
+
+
+def test_captures_leave_the_stream_as_it_was(dev):
+    """A model whose context works on a stream of its own: after a capture its
+    passes are on that stream again."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        ctx = capi.Context(0, stream=stream.cuda_stream)
+        m = QwenModel(ctx, CFG, synth.qwen_weights(CFG, 81, symmetric=True), max_batch=96)
+        stream.synchronize()
+        seen, call = [], m._call
+
+        def watched(name, *args):
+            if name == "gx_set_stream":
+                seen.append(args[1].value if hasattr(args[1], "value") else args[1])
+            return call(name, *args)
+
+        m._call = watched
+        m.set_pages(8, 16)
+        c = m.open_conversation()
+        m.forward_pages([prompt(119, 20)], [c])
+        m.start_pages([5], [c])
+        m.pages_step(graph=True)
+        m.capture_decode()
+        m.set_slots(2)
+        m.capture_slots(2)
+        assert len(seen) == 6 and seen[1::2] == [stream.cuda_stream] * 3
+        stream.synchronize()
+        m.free()
+        ctx.close()
