@@ -554,10 +554,14 @@ __global__ __launch_bounds__(64 * kWaves) void attn_paged_tile_kernel(const Args
 #pragma unroll
                 for (int i = 1; i < 8; i++)
                     mx = fmaxf(mx, s[i >> 2][i & 3]);
-                // (a row that sees nothing yet, or whose maximum has risen past what the
-                // reference allows: the reference becomes the maximum)
-                if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
-                    const float mn = fmaxf(m, groups_max(mx));
+                // (the reference of a row that sees nothing yet, or whose maximum has risen
+                // past what it allows, becomes the maximum; the others' stay: a row's bits
+                // hang on its own keys alone)
+                auto rises = [&](float to) __attribute__((always_inline)) {
+                    return to * x.c > m * x.c + kRise || (m == -INFINITY && to > m);
+                };
+                if (__ballot(rises(mx))) {
+                    const float most = groups_max(mx), mn = rises(most) ? most : m;
                     const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
                     m = mn;
                     l *= corr;
@@ -571,11 +575,11 @@ __global__ __launch_bounds__(64 * kWaves) void attn_paged_tile_kernel(const Args
                     for (int i = 0; i < 8; i++)
                         top = fmaxf(top, fabsf(sv[i]));  // (NaN falls out)
                     if (__ballot(top > cap)) {
-                        top = fmaxf(cap, groups_max(top));
-                        const float up = power_above(top);
+                        top = groups_max(top);
+                        const float up = top > cap ? power_above(top) : cap;
                         const float corr = cap == up ? 1.0f : cap / up;
                         cap = up;
-                        by = 1.0f / up;
+                        by = corr == 1.0f ? by : 1.0f / up;
 #pragma unroll
                         for (int d = 0; d < D; d++)
                             o[d] *= corr;
@@ -954,10 +958,10 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void attn_paged_wide_kernel(con
         for (int i = 1; i < 32; i++)
             mx = fmaxf(mx, s[i >> 4][i & 15]);
         mx = halves_max(mx);
-        // (a row that sees nothing yet, or whose maximum has risen past what the
-        // reference allows: the reference becomes the maximum)
-        if (__ballot(mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m))) {
-            const float mn = fmaxf(m, mx);
+        // (as in the kernel for few rows)
+        const bool rises = mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m);
+        if (__ballot(rises)) {
+            const float mn = rises ? mx : m;
             const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
             m = mn;
             l *= corr;
@@ -978,9 +982,9 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void attn_paged_wide_kernel(con
                 top = fmaxf(0.0f, wave_max(fabsf(scales[(2 * slot + 1) * kStage + lane])));
             }
             if (__ballot(top > cap)) {
-                const float up = power_above(fmaxf(cap, top)), corr = cap == up ? 1.0f : cap / up;
+                const float up = top > cap ? power_above(top) : cap, corr = cap == up ? 1.0f : cap / up;
                 cap = up;
-                by = 1.0f / up;
+                by = corr == 1.0f ? by : 1.0f / up;
 #pragma unroll
                 for (int et = 0; et < ET; et++)
                     o[et] *= corr;

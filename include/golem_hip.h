@@ -784,7 +784,8 @@ int gx_qwen_attention_paged_workspace_bytes(int n, int M, int max_tokens, int he
  * Lengths past max_length (at most table_width * page_size) are cut to it, tokens
  * past max_tokens left out; a token that sees a page outside the pool gets NaN.
  * Positions that a token does not see, whatever they hold, leave no trace in its
- * row.  Sizes are read on the device and nothing allocates: a captured call
+ * row, but infinite or NaN fp16 values of its conversation's later tokens: its
+ * sums are then taken again in another order, which moves their rounding.  Sizes are read on the device and nothing allocates: a captured call
  * may be replayed for other tokens, lengths and tables within its bounds.
  * workspace: 256-byte aligned; calls that may overlap need one each. */
 int gx_qwen_attention_paged(gx_ctx *ctx, const uint16_t *qh, int n, int M, int max_tokens, const int32_t *first,

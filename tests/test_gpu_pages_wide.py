@@ -121,3 +121,9 @@ def test_shared_pages(dev, wide):
 
 def test_none(dev, wide):
     base.test_attention_none(dev)
+
+
+@BITS
+@pytest.mark.parametrize("counts,lengths", [([9], [200]), ([150], [300]), ([40], [1500]), ([3, 35], [2300, 2100])])
+def test_large_hidden_scores_leave_no_trace(dev, wide, counts, lengths, bits):
+    base.test_attention_large_hidden_scores_leave_no_trace(dev, counts, lengths, bits)
