@@ -23,7 +23,8 @@
 // which the float output could not hide.
 //
 // 8-bit pages enter as fp16 integers, which are exact; a key's scale multiplies
-// its score, a value's its probability, each in float32.
+// its score, a value's its probability, each in float32.  What is cut in two is then
+// that product: within 2^-21 of it, or 2^-29 of the row's largest.
 #include <algorithm>
 #include <type_traits>
 
@@ -118,10 +119,36 @@ __device__ __forceinline__ float halves_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// The power of two above a scale (at most 2^127, whose inverse is no normal
-// number but exact).
-__device__ __forceinline__ float power_above(float top) {
-    return __uint_as_float(min((__float_as_uint(top) & 0x7F800000u) + 0x00800000u, 0x7F000000u));
+// What is added to a score in base 2, the reference m being in the scores' own units.
+__device__ __forceinline__ float base_of(float m, float c) { return kShift - (m == -INFINITY ? 0.0f : m * c); }
+
+// 8-bit values' scales go with the probabilities, z = p * scale, and those enter the
+// products as z / cap: cap is a power of two of a row's own, 2^-8 of its largest z,
+// and follows that as the maximum's reference does, when it rises past 2^15 cap or
+// the reference moves (so that a large scale with little weight, or one whose weight
+// has become little, takes no bits from the others).
+//
+// May a step's z pass 2^15 cap?  (r: its largest scale / cap, p: its largest
+// probability.  Nor may r itself come near float's largest, as p may be zero.)
+__device__ __forceinline__ bool cap_short(float r, float p) { return p * r > 0x1p15f || r > 0x1p100f; }
+// 2^-16 z, which float holds whatever the scale.
+__device__ __forceinline__ float scaled_down(float p, float scale) { return p * (fabsf(scale) * 0x1p-16f); }
+// A power of two above (at most 2^127), and one not above.
+__device__ __forceinline__ float power_above(float v) {
+    return __uint_as_float(min((__float_as_uint(v) & 0x7F800000u) + 0x00800000u, 0x7F000000u));
+}
+__device__ __forceinline__ float power_within(float v) { return __uint_as_float(__float_as_uint(v) & 0x7F800000u); }
+// A row's cap and its inverse, its sums being multiplied by corr for a reference that
+// moved; z: 2^-16 of the step's largest, or up to four times as much,
+// top: its largest scale.  Returns what the outputs, held divided by cap, are
+// multiplied by.
+__device__ __forceinline__ float cap_to(float &cap, float &by, float corr, bool moved, float z, float top) {
+    if (!moved && !(z > 0.5f * cap) && !(top * by > 0x1p100f))
+        return corr;
+    const float had = cap * corr;
+    cap = fminf(fmaxf(fmaxf(power_above(z) * 0x1p8f, power_within(had)), power_above(top) * 0x1p-100f), 0x1p126f);
+    by = __uint_as_float(0x7F000000u - __float_as_uint(cap));  // 1 / cap
+    return had * by;
 }
 
 // Two of eight bytes (w's four, then v's), integers, as fp16: set in the low bits of
@@ -469,7 +496,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_paged_tile_kernel(const Args
         const int r = min(r0 + li, R - 1), node = r / group, sees = t.sees(r, group);
         v4f o[D] = {};
         float m = -INFINITY, l = 0.0f;  // m: in the scores' own units
-        float cap = 0.0f, by = 0.0f;    // 8-bit values' outputs are held divided by cap, a power of two over their scales
+        float cap = 0.0f, by = 0.0f;    // 8-bit values' outputs are held divided by cap (by: 1 / cap)
         int j = t0 + wave;
         if (j < t1) {
             K k;
@@ -560,32 +587,33 @@ __global__ __launch_bounds__(64 * kWaves) void attn_paged_tile_kernel(const Args
                 auto rises = [&](float to) __attribute__((always_inline)) {
                     return to * x.c > m * x.c + kRise || (m == -INFINITY && to > m);
                 };
-                if (__ballot(rises(mx))) {
+                float top = 0.0f;
+                bool grows = false;
+                if constexpr (KIND == GX_PAGES_I8) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        top = fmaxf(top, fabsf(sv[i]));  // (NaN falls out)
+                    grows = cap_short(top * by, __builtin_amdgcn_exp2f(fmaf(mx, x.c, base_of(m, x.c))));
+                }
+                if (__ballot(rises(mx) || grows)) {
                     const float most = groups_max(mx), mn = rises(most) ? most : m;
-                    const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
-                    m = mn;
+                    float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
                     l *= corr;
+                    if constexpr (KIND == GX_PAGES_I8) {
+                        float base = base_of(mn, x.c);
+                        asm volatile("" : "+v"(base));  // (the branch's own probabilities)
+                        float z = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            z = fmaxf(z, scaled_down(__builtin_amdgcn_exp2f(fmaf(s[i >> 2][i & 3], x.c, base)), sv[i]));
+                        corr = cap_to(cap, by, corr, mn != m, groups_max(z), groups_max(top));
+                    }
+                    m = mn;
 #pragma unroll
                     for (int d = 0; d < D; d++)
                         o[d] *= corr;
                 }
-                if constexpr (KIND == GX_PAGES_I8) {
-                    float top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        top = fmaxf(top, fabsf(sv[i]));  // (NaN falls out)
-                    if (__ballot(top > cap)) {
-                        top = groups_max(top);
-                        const float up = top > cap ? power_above(top) : cap;
-                        const float corr = cap == up ? 1.0f : cap / up;
-                        cap = up;
-                        by = corr == 1.0f ? by : 1.0f / up;
-#pragma unroll
-                        for (int d = 0; d < D; d++)
-                            o[d] *= corr;
-                    }
-                }
-                const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
+                const float base = base_of(m, x.c);
                 float part = 0.0f, p[8];
                 uint32_t hb[4], lb[4];
 #pragma unroll
@@ -960,17 +988,9 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void attn_paged_wide_kernel(con
         mx = halves_max(mx);
         // (as in the kernel for few rows)
         const bool rises = mx * x.c > m * x.c + kRise || (m == -INFINITY && mx > m);
-        if (__ballot(rises)) {
-            const float mn = rises ? mx : m;
-            const float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
-            m = mn;
-            l *= corr;
-#pragma unroll
-            for (int et = 0; et < ET; et++)
-                o[et] *= corr;
-        }
+        float top = 0.0f, scale = 0.0f;
+        bool grows = false;
         if constexpr (!f16) {
-            float top = 0.0f;
             if (edge) {
 #pragma unroll
                 for (int i = 0; i < 32; i++) {
@@ -979,18 +999,42 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void attn_paged_wide_kernel(con
                 }
                 top = halves_max(top);
             } else {
-                top = fmaxf(0.0f, wave_max(fabsf(scales[(2 * slot + 1) * kStage + lane])));
+                scale = fabsf(scales[(2 * slot + 1) * kStage + lane]);
+                top = fmaxf(0.0f, wave_max(scale));
             }
-            if (__ballot(top > cap)) {
-                const float up = top > cap ? power_above(top) : cap, corr = cap == up ? 1.0f : cap / up;
-                cap = up;
-                by = corr == 1.0f ? by : 1.0f / up;
-#pragma unroll
-                for (int et = 0; et < ET; et++)
-                    o[et] *= corr;
-            }
+            grows = cap_short(top * by, __builtin_amdgcn_exp2f(fmaf(mx, x.c, base_of(m, x.c))));
         }
-        const float base = kShift - (m == -INFINITY ? 0.0f : m * x.c);
+        if (__ballot(rises || grows)) {
+            const float mn = rises ? mx : m;
+            float corr = mn == m ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * x.c);
+            l *= corr;
+            if constexpr (!f16) {
+                // z by the largest probability and the largest scale where the step's scales
+                // are within four of each other, or else key by key (for all: an 8-bit
+                // prompt of 2048 96 us, so 84)
+                float base = base_of(mn, x.c);
+                asm volatile("" : "+v"(base)::"memory");  // (the branch's own: no room to hold the step's over it)
+                float z = scaled_down(__builtin_amdgcn_exp2f(fmaf(mx, x.c, base)), top);
+                if (edge || !(-wave_max(-scale) * 4.0f >= top)) {
+                    asm volatile("" ::: "memory");  // (a branch)
+                    z = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float y = scaled_down(__builtin_amdgcn_exp2f(fmaf(s[i >> 4][i & 15], x.c, base)),
+                                                    vs[16 * (i >> 3) + (i & 7)]);
+                        z = fmaxf(z, edge && 16 * (i >> 3) + (i & 7) >= lim ? 0.0f : y);
+                    }
+                    z = halves_max(z);
+                }
+                asm volatile("" ::: "memory");
+                corr = cap_to(cap, by, corr, mn != m, z, top);
+            }
+            m = mn;
+#pragma unroll
+            for (int et = 0; et < ET; et++)
+                o[et] *= corr;
+        }
+        const float base = base_of(m, x.c);
         v8h ph[4], pl[4];
         // eight keys' probabilities (times their values' scales), their leading 11 bits and the rest
         auto chances = [&](int w) __attribute__((always_inline)) {

@@ -778,15 +778,18 @@ int gx_qwen_attention_paged_workspace_bytes(int n, int M, int max_tokens, int he
  * positions; a token at position p sees positions 0 .. p of its conversation.
  * For query head h and the positions j it sees, s_j = q . k_j / sqrt(head_dim):
  *   o = sum_j e^(s_j) v_j / sum_j e^(s_j)
- * in float; a token before position 0 (more tokens than positions) sees none and
- * gets zeros.  out [M][heads * head_dim] floats and the Q8_0 form q/scales/qsum
- * (either may be NULL).  Rows outside every conversation are left as they were.
- * Lengths past max_length (at most table_width * page_size) are cut to it, tokens
- * past max_tokens left out; a token that sees a page outside the pool gets NaN.
+ * in float, each e^(s_j), for 8-bit pages times its value's scale, within 2^-21 of
+ * itself or 2^-29 of the row's largest; a token before position 0 (more tokens than
+ * positions) sees none and gets zeros.  out [M][heads * head_dim] floats and the
+ * Q8_0 form q/scales/qsum (either may be NULL).  Rows outside every conversation are
+ * left as they were.  Lengths past max_length (at most table_width * page_size) are
+ * cut to it, tokens past max_tokens left out (those before them then stand at the
+ * last positions); a token that sees a page outside the pool gets NaN.
  * Positions that a token does not see, whatever they hold, leave no trace in its
  * row, but infinite or NaN fp16 values of its conversation's later tokens: its
- * sums are then taken again in another order, which moves their rounding.  Sizes are read on the device and nothing allocates: a captured call
- * may be replayed for other tokens, lengths and tables within its bounds.
+ * sums are then taken again in another order, which moves their rounding.  Sizes
+ * are read on the device and nothing allocates: a captured call may be replayed for
+ * other tokens, lengths and tables within its bounds.
  * workspace: 256-byte aligned; calls that may overlap need one each. */
 int gx_qwen_attention_paged(gx_ctx *ctx, const uint16_t *qh, int n, int M, int max_tokens, const int32_t *first,
                             const int32_t *lengths, int max_length, int heads, int kv_heads, int head_dim, int kind,

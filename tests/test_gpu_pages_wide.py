@@ -127,3 +127,10 @@ def test_none(dev, wide):
 @pytest.mark.parametrize("counts,lengths", [([9], [200]), ([150], [300]), ([40], [1500]), ([3, 35], [2300, 2100])])
 def test_large_hidden_scores_leave_no_trace(dev, wide, counts, lengths, bits):
     base.test_attention_large_hidden_scores_leave_no_trace(dev, counts, lengths, bits)
+
+
+@FORMS
+@pytest.mark.parametrize("near", [0, 1])
+@pytest.mark.parametrize("grow", [20, 60, 110])
+def test_large_scales_of_small_weight(dev, wide, counts, lengths, near, grow):
+    base.test_attention_large_scales_of_small_weight(dev, counts, lengths, near, grow)
