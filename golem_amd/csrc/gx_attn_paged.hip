@@ -164,10 +164,10 @@ __device__ __forceinline__ uint32_t bytes_to_half(uint32_t turned) {
 
 // A step's keys as they come from the pages, 1 KiB an instruction in whole lines,
 // and through a wavefront's own LDS to the lanes that want them: a product's
-// sixteen keys read where they lie are 64 bytes each of sixteen lines, which took
-// the loads of 64 conversations from 120 us to 140 (8-bit pages 69 to 90).  Pieces
-// of 16 bytes are exchanged by the key, or rows padded where they are no power of
-// two, so that sixteen keys' pieces go round the banks.
+// sixteen keys read where they lie are 64 bytes each of sixteen lines (one token
+// after 500 positions 9.9 us so, 7.0 by LDS).  Pieces of 16 bytes are exchanged by
+// the key, or rows padded where they are no power of two, so that sixteen keys'
+// pieces go round the banks.
 template <int HD, int KIND>
 struct Keys {
     static constexpr int RB = HD * (KIND == GX_PAGES_F16 ? 2 : 1), CH = RB / 16, N = CH / 2, KS = HD / 32;
@@ -733,10 +733,10 @@ __global__ __launch_bounds__(64 * kWaves) void attn_paged_tile_kernel(const Args
 // round the banks.  fp16 pages come in by direct loads, one step ahead of the
 // products; 8-bit ones through registers, two steps ahead, made fp16 on the way.
 // Tiles that see most come first, and then those that see least: with two
-// workgroups a CU the long ones lie beside the short ones (a prompt of 2048 68 us;
+// workgroups a CU the long ones lie beside the short ones (a prompt of 2048 65 us;
 // long and short in turn 77).
 //
-// A prompt of 2048 tokens of 32 heads over 8 of 128 takes 68 to 70 us, 34 GFLOP:
+// A prompt of 2048 tokens of 32 heads over 8 of 128 takes 64 to 69 us by card, 34 GFLOP:
 // the longest tile's 32 steps after each other, 2 us each on a CU of its own; two
 // workgroups a CU take 3.5 us for a step of each, where the matrix instructions
 // alone (96 a SIMD, a third of them for the probabilities' second part) take 2.1 at
@@ -1269,22 +1269,25 @@ struct Plan {
     int S, G, least;
 };
 
-// Which kernel, and how it is launched, by what each would take (us, as measured at
-// 32 query heads over 8 of 128, fp16):
+// Which kernel, and how it is launched.  The times (us) are of 32 query heads over 8
+// of 128, fp16, thirty calls over the same pages; over three sets of pages in turn
+// they are up to a fifth longer.  The rule goes by these for every width and kind.
 //
-// A tile of 16 rows a workgroup takes 6 and 1.1 a round of eight steps, one of its
-// workgroups a CU (1.7 where the tiles are more than the CUs): 9 tokens of one
-// conversation after 500 positions 7.9, 17 of eight after 1000 11.5, 33 after 4000
-// 23.  The kernel for many rows takes 4, 2 a step and, in shares, 6 for the join
-// and its parts' bytes at 4 TB/s: 15, 19 and 18 for the same three, 48 for a prompt
-// of 1024 where the tiles take 56.
+// Many rows or tiles, by estimates.  A tile of 16 rows a workgroup takes 6 and 1.1 a
+// round of eight steps, one of its workgroups a CU (1.7 where the tiles are more than
+// the CUs): 9 tokens of one conversation after 500 positions 7.9, 17 of eight after
+// 1000 11.5, 33 after 4000 23, a prompt of 1024 56.  The kernel for many rows takes
+// 4, 2 a step and, in shares, 6 for the join and its parts' bytes at 4 TB/s: 15, 19,
+// 17 and 33 for the same four.  Near the border it misses: a prompt of 512 takes 24
+// by tiles, as chosen, and 21 by the other; at 64 wide one of 1024 takes 39, as
+// chosen, and 29 by tiles.  Widths 32 and 96 have the tiles alone.
 //
-// The tiles' steps are spread, which costs the search for a workgroup's part and
-// the join, where whole tiles would leave CUs idle for long: one token after 1000
-// positions 9.3 whole and 11.0 spread, after 1600 11.5 either way, after 4000 22.1
-// and 12.9; four after 1000 9.9 and 13.6, after 2000 17.7 and 13.9; 12 after 4000
-// 39.7 and 39.0, 16 42.2 and 46.2 (8-bit 30.7 and 28.9).  64 of up to 4000 take 139
-// either way; past that the longest one would be alone at the end.
+// Whole tiles or their steps spread, by thresholds.  Spreading costs the search for a
+// workgroup's part and the join, and pays where whole tiles would leave CUs idle for
+// long: one token after 1000 positions 9.2 whole and 10.6 spread, after 1600 11.9 and
+// 11.5, after 4000 28.6 and 12.1; four after 1000 10.9 and 12.8, after 2000 17.7 and
+// 13.8; 12 after 4000 39.4 and 37.7, 16 41.6 and 45.5 (8-bit 31.6 and 29.3), 64 138
+// and 137.  Past 256 steps the longest conversation would be alone at the end.
 Plan plan_of(int n, int M, int max_tokens, int heads, int kv_heads, int hd, int max_length) {
     const int64_t rows = (int64_t)max_tokens * (heads / kv_heads), all = (int64_t)kv_heads * std::max(n, 1);
     const int64_t tiles = (rows + kRows - 1) / kRows, steps = (max_length + (int64_t)kKeys - 1) / kKeys;

@@ -713,7 +713,8 @@ int gx_qwen_cache_fork(gx_ctx *ctx, int layers, uint16_t *const *kcaches, uint16
  *                   or int8 (GX_PAGES_I8)
  *   their scales    float [pages][kv_heads][page_size] (GX_PAGES_I8; else NULL):
  *                   a head's vector at a position stands for scale * int8,
- *                   the scale finite, or NaN for a vector that is all NaN
+ *                   the scale finite, or NaN for a vector that is all NaN (values
+ *                   past 2^90 may leave the range of the attention's sums)
  *   table           int32 [n][table_width]: conversation b's position p lies in
  *                   page table[b][p / page_size] at p % page_size
  * A page may stand in several conversations' rows (a common beginning), as long
